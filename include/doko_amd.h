@@ -624,6 +624,78 @@ int dk_net_gelu_bias_f32_async(void* y, const void* bias, uint64_t n, uint32_t w
 int dk_net_attn62_bias_f32_async(const void* qkv, const void* bqkv, void* y, uint32_t batch, uint32_t heads,
                                  uint32_t head_dim, void* stream);
 
+/* ---- training operators: LayerNorm with its gradient, log probabilities with theirs, AdamW -------
+ * What a training step of the networks chains (az_doko.py's fit: norm, loss, update).  Each call runs
+ * on the caller's stream, allocates and synchronises nothing and may be captured into a graph.  Element
+ * types are dk_net_type; every sum and statistic is f32.  Strides are in elements between rows; the
+ * last dimension is dense and rows need no alignment beyond their elements'. */
+enum dk_net_type { DK_F32 = 0, DK_BF16 = 1, DK_F16 = 2 };
+
+/* dk_net_layer_norm_async: x_out = x + delta (rounded to `type`), h_out = LayerNorm(x_out; gamma, beta,
+ * eps) over d <= 16384 columns; delta NULL: h_out = LayerNorm(x), x_out may be NULL.  gamma / beta are of
+ * `wtype` (DK_F32 or `type`), NULL for 1 / 0.  stats [rows][2] (or NULL) receives each row's mean and
+ * 1 / sqrt(var + eps) for the backward pass.  x_out and h_out are dense [rows][d]; x_out may be x, or delta
+ * where that is dense.
+ * dk_net_layer_norm_bwd_async: dh = the gradient of h_out, dx_res (or NULL) that of x_out, x the rows that
+ * were normalised; dx [rows][d] is the gradient of x (and of delta), dgamma / dbeta [d] (either may be
+ * NULL) are of `wtype`.  Without dgamma and dbeta the workspace may be NULL; otherwise it has
+ * dk_net_layer_norm_bwd_workspace(rows, d, type) bytes and is the call's own until it is done.  The
+ * reductions over the rows have a fixed order: equal inputs give equal bits. */
+int dk_net_layer_norm_async(const void* x, uint64_t x_stride, const void* delta, uint64_t delta_stride, uint64_t rows,
+                            uint32_t d, int type, const void* gamma, const void* beta, int wtype, float eps, void* x_out,
+                            void* h_out, float* stats, void* stream);
+uint64_t dk_net_layer_norm_bwd_workspace(uint64_t rows, uint32_t d, int type);
+int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* dx_res, uint64_t dx_res_stride, const void* x,
+                                uint64_t x_stride, const float* stats, uint64_t rows, uint32_t d, int type,
+                                const void* gamma, int wtype, void* dx, void* dgamma, void* dbeta, void* workspace,
+                                uint64_t workspace_bytes, void* stream);
+
+/* dk_net_token_logprobs_async: per row of logits [rows][vocab], with z = logits / temperature over the
+ * entries that mask [rows][vocab] (bytes, 0 = not allowed; NULL: all) allows:
+ *   logprobs [rows][n]    z[tokens[i]] - log sum e^z; 0 for a negative token (padding), -inf for one that is
+ *                         not allowed or holds -inf, NaN for one >= vocab (nothing is read there)
+ *   entropy [rows]        of the row's distribution (NULL: not wanted)
+ *   lse [rows]            log sum e^z, for the backward pass (NULL: not wanted)
+ *   top_logprobs, top_tokens [rows][top]   the largest by (logit descending, index ascending); where fewer are
+ *                         allowed -inf and -1
+ * n <= 64, top <= 32.  A row with nothing allowed has entropy 0 and lse -inf.  Whatever a masked entry
+ * holds is not looked at; a NaN or +inf in an allowed one makes the row's floating results NaN (its
+ * top_tokens are still tokens of the row, NaN never among them).
+ * mask_stride 0 applies one mask to every row.  The workspace has dk_net_token_logprobs_workspace bytes
+ * (which may be 0: then it may be NULL).
+ * dk_net_token_logprobs_bwd_async: dlogits (dense [rows][vocab], of `type`, not the logits' own buffer)
+ * from dlogprobs [rows][n] and dentropy [rows] (either may be NULL), with lse and entropy of the
+ * forward call.  A token given twice takes both gradients; padding, out-of-range and
+ * disallowed tokens take none, nor do disallowed entries. */
+int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t rows, uint32_t vocab, int type,
+                                const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
+                                uint32_t n, uint32_t top, float* logprobs, float* entropy, float* lse, float* top_logprobs,
+                                int64_t* top_tokens, void* workspace, uint64_t workspace_bytes, void* stream);
+uint64_t dk_net_token_logprobs_workspace(uint64_t rows, uint32_t vocab, int type, uint32_t top);
+int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_t rows, uint32_t vocab, int type,
+                                    const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
+                                    uint32_t n, const float* lse, const float* entropy, const float* dlogprobs,
+                                    const float* dentropy, void* dlogits, void* stream);
+
+/* dk_net_adamw_async: one AdamW step of `count` tensors (host array; dense parameters and gradients of
+ * `type`).  A tensor's states are the blocks of 256 elements from `block` on in the flat buffers; no block
+ * belongs to two tensors.  state_bits 32: exp_avg / exp_avg_sq are f32.  state_bits 8: e4m3 codes of exp_avg
+ * and of sqrt(exp_avg_sq), times one f32 scale for each block.  master (or NULL): f32 weights laid out as the states;
+ * the step is theirs and p receives them rounded.  step (int32) and factors (3 floats, scratch) are indexed
+ * by `id`: step[id] counts on the device, so that a captured step goes on counting.  d_lr (or NULL) is
+ * read on the device in place of lr. */
+typedef struct dk_net_adamw_tensor {
+    void* p;
+    const void* g;
+    uint64_t n;
+    uint64_t block;
+    uint64_t id;
+} dk_net_adamw_tensor;
+int dk_net_adamw_async(const dk_net_adamw_tensor* tensors, uint32_t count, int type, int state_bits, void* exp_avg,
+                       void* exp_avg_sq, float* exp_avg_scale, float* exp_avg_sq_scale, float* master, int32_t* step,
+                       float* factors, double lr, const float* d_lr, double beta1, double beta2, double eps,
+                       double weight_decay, void* stream);
+
 /* ---- completion / errors / timing of *_async work -------------------------------
  * dk_sync: waits for the stream and returns the first device-side error
  * (DK_E_CAPACITY when a search ran out of child slots) since the last dk_sync, including

@@ -19,6 +19,16 @@ __all__ = ["Engine", "McEnv", "CachedMCTS", "SmallRng", "card_matching_full", "s
            "fdo_from_fields", "fdo_to_fields", "do_from_fields", "do_to_fields", "ttt_state",
            "tic_tac_toe_player", "tic_tac_toe_games"]
 
+# the networks' training operators (net_ops.py), on first use: the search alone does not need torch
+_NET_OPS = ("layer_norm", "token_logprobs", "TokenLogprobs", "AdamW")
+
+
+def __getattr__(name):
+    if name in _NET_OPS:
+        from . import net_ops
+        return getattr(net_ops, name)
+    raise AttributeError("module %r has no attribute %r" % (__name__, name))
+
 
 def build(verbose=False):
     return _native.build(verbose=verbose)

@@ -6,6 +6,7 @@ is usable, the product API raises.
 import ctypes
 import os
 import subprocess
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -13,24 +14,35 @@ LIB_PATH = os.path.join(PKG_DIR, "libdoko_amd.so")
 # profiling builds (-DDK_PHASE_PROF) are loaded by setting DK_LIB to their path
 PROF_LIB_PATH = os.path.join(PKG_DIR, "libdoko_amd_prof.so")
 SRC = os.path.join(PKG_DIR, "csrc", "doko_amd.hip")
+TRAIN_SRC = os.path.join(PKG_DIR, "csrc", "net_train.hip")
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared"]
+# the training operators: no packed f32 instructions (the host pass warns that it does not know the feature)
+TRAIN_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def build(verbose=False, profiling=False):
-    """Compile csrc/doko_amd.hip for gfx950 into the package directory (in-tree).
-    profiling=True builds the phase-timer variant libdoko_amd_prof.so."""
+    """Compile csrc/net_train.hip and csrc/doko_amd.hip for gfx950 and link them in the package directory
+    (in-tree).  profiling=True builds the phase-timer variant libdoko_amd_prof.so."""
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     out = PROF_LIB_PATH if profiling else LIB_PATH
-    cmd = [hipcc] + HIPCC_FLAGS + (["-DDK_PHASE_PROF"] if profiling else []) + ["-o", out, SRC]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True, cwd=PKG_DIR)
+    with tempfile.TemporaryDirectory() as tmp:
+        obj = os.path.join(tmp, "net_train.o")
+        for cmd in ([hipcc] + TRAIN_FLAGS + ["-c", "-o", obj, TRAIN_SRC],
+                    [hipcc] + HIPCC_FLAGS + (["-DDK_PHASE_PROF"] if profiling else []) + ["-o", out, SRC, obj]):
+            if verbose:
+                print(" ".join(cmd))
+            subprocess.run(cmd, check=True, cwd=PKG_DIR)
     return out
 
 
 class dk_config(ctypes.Structure):
     _fields_ = [("device", ctypes.c_int32), ("max_roots", ctypes.c_uint32),
                 ("max_iterations", ctypes.c_uint32), ("slot_capacity", ctypes.c_uint32)]
+
+
+class dk_net_adamw_tensor(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("n", ctypes.c_uint64), ("block", ctypes.c_uint64),
+                ("id", ctypes.c_uint64)]
 
 
 _lib = None
@@ -136,6 +148,18 @@ def lib():
         "dk_net_add_bias_ln_f32_async": (ctypes.c_int, [vp, vp, vp, u32, u32, vp, vp, ctypes.c_float, vp, vp]),
         "dk_net_gelu_bias_f32_async": (ctypes.c_int, [vp, vp, u64, u32, vp]),
         "dk_net_attn62_bias_f32_async": (ctypes.c_int, [vp, vp, vp, u32, u32, u32, vp]),
+        "dk_net_layer_norm_async": (ctypes.c_int, [vp, u64, vp, u64, u64, u32, ctypes.c_int, vp, vp, ctypes.c_int, ctypes.c_float,
+                                                   vp, vp, vp, vp]),
+        "dk_net_layer_norm_bwd_workspace": (u64, [u64, u32, ctypes.c_int]),
+        "dk_net_layer_norm_bwd_async": (ctypes.c_int, [vp, u64, vp, u64, vp, u64, vp, u64, u32, ctypes.c_int, vp, ctypes.c_int, vp,
+                                                       vp, vp, vp, u64, vp]),
+        "dk_net_token_logprobs_async": (ctypes.c_int, [vp, u64, u64, u32, ctypes.c_int, vp, u64, ctypes.c_float, vp, u32, u32, vp,
+                                                       vp, vp, vp, vp, vp, u64, vp]),
+        "dk_net_token_logprobs_workspace": (u64, [u64, u32, ctypes.c_int, u32]),
+        "dk_net_token_logprobs_bwd_async": (ctypes.c_int, [vp, u64, u64, u32, ctypes.c_int, vp, u64, ctypes.c_float, vp, u32, vp, vp,
+                                                           vp, vp, vp, vp]),
+        "dk_net_adamw_async": (ctypes.c_int, [vp, u32, ctypes.c_int, ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, ctypes.c_double, vp,
+                                              ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)
@@ -159,5 +183,6 @@ EXPORTED = [
     "dk_net_embed_ln_f32_async", "dk_net_add_ln_f32_async", "dk_net_attn62_f32_async", "dk_net_gelu_f32_async", "dk_net_add_bias_ln_f32_async", "dk_net_gelu_bias_f32_async", "dk_net_attn62_bias_f32_async", "dk_ar_begin_async", "dk_ar_guesses_async", "dk_ar_prepare_async",
     "dk_ar_choose_async", "dk_ar_output_async", "dk_ar_fallback_async", "dk_fuse_accumulate_masked_async",
     "dk_fdo_from_fields", "dk_fdo_to_fields", "dk_do_from_fields", "dk_do_to_fields", "dk_is_consistent_batch",
-    "dk_pool_high_water",
+    "dk_pool_high_water", "dk_net_layer_norm_async", "dk_net_layer_norm_bwd_workspace", "dk_net_layer_norm_bwd_async",
+    "dk_net_token_logprobs_async", "dk_net_token_logprobs_workspace", "dk_net_token_logprobs_bwd_async", "dk_net_adamw_async",
 ]

@@ -1,0 +1,199 @@
+// The training operators of include/doko_amd.h (dk_net_layer_norm_*, dk_net_token_logprobs_*,
+// dk_net_adamw_async): argument checks and launches of the kernels in train_*_kernels.h.  A translation
+// unit of its own, linked into libdoko_amd.so.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdio>
+
+#include "../../include/doko_amd.h"
+#include "train_adamw_kernels.h"
+#include "train_logp_kernels.h"
+#include "train_norm_kernels.h"
+
+namespace {
+
+using namespace dk::train;
+
+#define DK_HIP(call)                                              \
+    do {                                                          \
+        hipError_t e_ = (call);                                   \
+        if (e_ != hipSuccess) {                                   \
+            fprintf(stderr, "doko_amd: %s failed: %s (%s:%d)\n", #call, hipGetErrorString(e_), __FILE__, __LINE__); \
+            return DK_E_LAUNCH;                                   \
+        }                                                         \
+    } while (0)
+
+constexpr uint32_t NORM_MAX_D = 16384;
+constexpr uint64_t MAX_GRID = 0x7FFFFFFFull;
+
+bool type_ok(int t) { return t == DK_F32 || t == DK_BF16 || t == DK_F16; }
+
+// calls f with a value of the element type `type` names
+template <class F>
+void with_type(int type, F f) {
+    if (type == DK_F32) f(float{});
+    else if (type == DK_BF16) f(__bf16{});
+    else f(_Float16{});
+}
+// the same for a weight: f32, or the activations' type T
+template <class T, class F>
+void with_weight(int wtype, F f) {
+    if (wtype == DK_F32) f(float{});
+    else f(T{});
+}
+
+constexpr uint32_t norm_slices(uint64_t rows) { return rows >= 64u * 64u ? 64u : rows ? (uint32_t)((rows + 63u) / 64u) : 1u; }
+
+}  // namespace
+
+extern "C" {
+
+int dk_net_layer_norm_async(const void* x, uint64_t x_stride, const void* delta, uint64_t delta_stride, uint64_t rows,
+                            uint32_t d, int type, const void* gamma, const void* beta, int wtype, float eps, void* x_out,
+                            void* h_out, float* stats, void* stream) {
+    if (!type_ok(type) || (wtype != DK_F32 && wtype != type) || d == 0 || d > NORM_MAX_D || (delta && !x_out) ||
+        rows > MAX_GRID)
+        return DK_E_INVALID;
+    if (rows == 0) return DK_OK;
+    if (!x || !h_out) return DK_E_INVALID;
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        with_weight<T>(wtype, [&](auto w) {
+            using W = decltype(w);
+            hipLaunchKernelGGL((layer_norm_kernel<T, W>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream,
+                               (const T*)x, x_stride, (const T*)delta, delta_stride, rows, d, (const W*)gamma,
+                               (const W*)beta, eps, (T*)x_out, (T*)h_out, stats);
+        });
+    });
+    DK_HIP(hipGetLastError());
+    return DK_OK;
+}
+
+uint64_t dk_net_layer_norm_bwd_workspace(uint64_t rows, uint32_t d, int type) {
+    (void)type;
+    return (uint64_t)norm_slices(rows) * 2 * d * sizeof(float);
+}
+
+int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* dx_res, uint64_t dx_res_stride, const void* x,
+                                uint64_t x_stride, const float* stats, uint64_t rows, uint32_t d, int type,
+                                const void* gamma, int wtype, void* dx, void* dgamma, void* dbeta, void* workspace,
+                                uint64_t workspace_bytes, void* stream) {
+    if (!type_ok(type) || (wtype != DK_F32 && wtype != type) || d == 0 || d > NORM_MAX_D || rows > MAX_GRID)
+        return DK_E_INVALID;
+    if (rows && (!dh || !x || !stats || !dx)) return DK_E_INVALID;
+    const bool weights = dgamma || dbeta;
+    if (weights && (!workspace || workspace_bytes < dk_net_layer_norm_bwd_workspace(rows, d, type))) return DK_E_INVALID;
+    if (rows == 0 && !weights) return DK_OK;
+    hipStream_t st = (hipStream_t)stream;
+    const uint32_t slices = norm_slices(rows);
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        with_weight<T>(wtype, [&](auto w) {
+            using W = decltype(w);
+            if (rows)
+                hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st,
+                                   (const T*)dh, dh_stride, (const T*)dx_res, dx_res_stride, (const T*)x, x_stride, stats,
+                                   rows, d, (const W*)gamma, (T*)dx);
+            if (weights) {
+                if (rows)
+                    hipLaunchKernelGGL(layer_norm_dw_kernel<T>, dim3((d + 63) / 64, slices), dim3(256), 0, st,
+                                       (const T*)dh, dh_stride, (const T*)x, x_stride, stats, rows, d,
+                                       (rows + slices - 1) / slices, (float*)workspace);
+                hipLaunchKernelGGL(layer_norm_dw_join_kernel<W>, dim3((2 * d + 255) / 256), dim3(256), 0, st,
+                                   (const float*)workspace, rows ? slices : 0u, d, (W*)dgamma, (W*)dbeta);
+            }
+        });
+    });
+    DK_HIP(hipGetLastError());
+    return DK_OK;
+}
+
+int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t rows, uint32_t vocab, int type,
+                                const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
+                                uint32_t n, uint32_t top, float* logprobs, float* entropy, float* lse, float* top_logprobs,
+                                int64_t* top_tokens, void* workspace, uint64_t workspace_bytes, void* stream) {
+    (void)workspace;
+    (void)workspace_bytes;
+    if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || top > TOP_MAX || rows > MAX_GRID ||
+        !(temperature > 0.0f) || std::isinf(temperature))
+        return DK_E_INVALID;
+    if (rows == 0) return DK_OK;
+    if (!logits || (n && (!tokens || !logprobs)) || (top && (!top_logprobs || !top_tokens))) return DK_E_INVALID;
+    const LogpArgs a{logits, stride, rows, vocab, n, top, mask, mask_stride, 1.0f / temperature, tokens, logprobs, entropy,
+                     lse, top_logprobs, top_tokens};
+    with_type(type, [&](auto t) {
+        hipLaunchKernelGGL(token_logprobs_kernel<decltype(t)>, dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);
+    });
+    DK_HIP(hipGetLastError());
+    return DK_OK;
+}
+
+uint64_t dk_net_token_logprobs_workspace(uint64_t rows, uint32_t vocab, int type, uint32_t top) {
+    (void)rows; (void)vocab; (void)type; (void)top;
+    return 0;
+}
+
+int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_t rows, uint32_t vocab, int type,
+                                    const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
+                                    uint32_t n, const float* lse, const float* entropy, const float* dlogprobs,
+                                    const float* dentropy, void* dlogits, void* stream) {
+    if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || rows > MAX_GRID || !(temperature > 0.0f) ||
+        std::isinf(temperature))
+        return DK_E_INVALID;
+    if (rows == 0) return DK_OK;
+    if (!logits || (n && !tokens) || !lse || !entropy || !dlogits) return DK_E_INVALID;
+    const LogpBwdArgs a{logits, stride, rows, vocab, n, mask, mask_stride, 1.0f / temperature, tokens, lse, entropy,
+                        dlogprobs, dentropy, dlogits};
+    with_type(type, [&](auto t) {
+        hipLaunchKernelGGL(token_logprobs_bwd_kernel<decltype(t)>, dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);
+    });
+    DK_HIP(hipGetLastError());
+    return DK_OK;
+}
+
+int dk_net_adamw_async(const dk_net_adamw_tensor* tensors, uint32_t count, int type, int state_bits, void* exp_avg,
+                       void* exp_avg_sq, float* exp_avg_scale, float* exp_avg_sq_scale, float* master, int32_t* step,
+                       float* factors, double lr, const float* d_lr, double beta1, double beta2, double eps,
+                       double weight_decay, void* stream) {
+    if (!type_ok(type) || (state_bits != 32 && state_bits != 8) || !(beta1 >= 0.0 && beta1 < 1.0) ||
+        !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0))
+        return DK_E_INVALID;
+    if (count == 0) return DK_OK;
+    if (!tensors || !exp_avg || !exp_avg_sq || !step || !factors || (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)))
+        return DK_E_INVALID;
+    for (uint32_t i = 0; i < count; ++i)
+        if ((tensors[i].n && (!tensors[i].p || !tensors[i].g)) || tensors[i].n > MAX_GRID * ADAMW_BLOCK) return DK_E_INVALID;
+    const AdamwArgs a{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, exp_avg, exp_avg_sq,
+                      exp_avg_scale, exp_avg_sq_scale, master, factors};
+    hipStream_t st = (hipStream_t)stream;
+    AdamwTable tab;
+    for (uint32_t at = 0; at < count;) {
+        uint32_t k = 0;
+        uint64_t groups = 0;
+        for (; k < ADAMW_TENSORS && at < count; ++k, ++at) {
+            const dk_net_adamw_tensor& t = tensors[at];
+            const uint64_t more = (t.n + 4 * ADAMW_BLOCK - 1) / (4 * ADAMW_BLOCK);
+            if (groups + more > MAX_GRID) break;
+            tab.p[k] = t.p; tab.g[k] = t.g; tab.n[k] = t.n; tab.block[k] = t.block; tab.id[k] = t.id;
+            tab.first[k] = (uint32_t)groups;
+            groups += more;
+        }
+        tab.count = k;
+        tab.first[k] = (uint32_t)groups;
+        hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(ADAMW_TENSORS), 0, st, tab, lr, d_lr, std::log(beta1),
+                           std::log(beta2), weight_decay, step, factors);
+        if (groups)
+            with_type(type, [&](auto t) {
+                using T = decltype(t);
+                if (state_bits == 8)
+                    hipLaunchKernelGGL((adamw_kernel<T, 8>), dim3((uint32_t)groups), dim3(256), 0, st, tab, a);
+                else
+                    hipLaunchKernelGGL((adamw_kernel<T, 32>), dim3((uint32_t)groups), dim3(256), 0, st, tab, a);
+            });
+        DK_HIP(hipGetLastError());
+    }
+    return DK_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,385 @@
+"""The operators of a training step on the GPU: LayerNorm with the residual add before it, log
+probabilities of given tokens with entropy and top alternatives, and AdamW over many tensors at once.
+
+Each is a HIP kernel behind the C-ABI (dk_net_layer_norm_*, dk_net_token_logprobs_*,
+dk_net_adamw_async; csrc/train_*_kernels.h) on torch's current stream of the tensors' device, and the
+first two are differentiable (once).  f32, bf16 and f16; sums and statistics are f32.  There is no CPU
+fallback.  DokoAzNet.loss / DokoImpiNet.loss are built on the first two, NetTrainer on all three.
+"""
+import math
+from typing import NamedTuple, Optional
+
+import numpy as np
+import torch
+
+from . import _native
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # enum dk_net_type
+NORM_MAX_D, TOKENS_MAX, TOP_MAX, ADAMW_BLOCK = 16384, 64, 32, 256
+
+
+def _check(rc, what):
+    if rc != 0:
+        raise RuntimeError("doko_amd %s kernel error %d" % (what, rc))
+
+
+def _launch(fn, device, *args):
+    """fn(*args, stream) on torch's current stream of `device`, with that device current."""
+    st = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        return fn(*args, st)
+    with torch.cuda.device(device):
+        return fn(*args, st)
+
+
+def _rows(t):
+    """t as rows over its last dimension: (2-D tensor with a dense last dimension, elements between rows).
+    Copies only what has no such view."""
+    r = t.reshape(-1, t.shape[-1])
+    if r.stride(1) != 1 and r.shape[1] > 1:
+        r = r.contiguous()
+    return r, r.stride(0)
+
+
+def _floating(t, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError("%s: a tensor on the GPU is needed" % what)
+    if t.dtype not in _TYPES:
+        raise ValueError("%s: float32, bfloat16 or float16 is needed, got %s" % (what, t.dtype))
+    return _TYPES[t.dtype]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ------------------------------------------------------------------------------- layer norm
+def _norm_forward(x, delta, weight, bias, eps, stats):
+    d = x.shape[-1]
+    xr, xs = _rows(x)
+    dr, ds = _rows(delta) if delta is not None else (None, 0)
+    rows = xr.shape[0]
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    new = torch.empty(x.shape, dtype=x.dtype, device=x.device) if delta is not None else None
+    st = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if stats else None
+    w = weight if weight is not None else bias
+    _check(_launch(_native.lib().dk_net_layer_norm_async, x.device, xr.data_ptr(), xs, _ptr(dr), ds, rows, d, _TYPES[x.dtype],
+                   _ptr(weight), _ptr(bias), _TYPES[w.dtype] if w is not None else 0, eps, _ptr(new), h.data_ptr(), _ptr(st)),
+           "layer norm")
+    return new, h, st, xr
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, delta, weight, bias, eps):
+        new, h, st, xr = _norm_forward(x, delta, weight, bias, eps, True)
+        ctx.shape, ctx.bias = x.shape, None if bias is None else bias.dtype
+        ctx.save_for_backward(new if new is not None else xr, st, weight)
+        ctx.set_materialize_grads(False)
+        return h if new is None else (new, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        dres, dh = (None, grads[0]) if len(grads) == 1 else grads
+        need_x, need_delta, need_w, need_b = ctx.needs_input_grad[:4]
+        if dh is None:
+            return (dres if need_x else None), (dres if need_delta else None), None, None, None
+        x, st, weight = ctx.saved_tensors
+        xr, xs = _rows(x)
+        rows, d = xr.shape
+        gr, gs = _rows(dh)
+        rr, rs = _rows(dres) if dres is not None else (None, 0)
+        wdtype = weight.dtype if weight is not None else ctx.bias if ctx.bias is not None else torch.float32
+        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty(d, dtype=wdtype, device=x.device) if need_w else None
+        db = torch.empty(d, dtype=wdtype, device=x.device) if need_b else None
+        L = _native.lib()
+        size = L.dk_net_layer_norm_bwd_workspace(rows, d, _TYPES[x.dtype]) if need_w or need_b else 0
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        _check(_launch(L.dk_net_layer_norm_bwd_async, x.device, gr.data_ptr(), gs, _ptr(rr), rs, xr.data_ptr(), xs, st.data_ptr(),
+                       rows, d, _TYPES[x.dtype], _ptr(weight), _TYPES[wdtype], dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), size),
+               "layer norm backward")
+        return (dx if need_x else None), (dx if need_delta else None), dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, delta=None):
+    """LayerNorm over the last dimension (at most 16384 columns), any leading dimensions and row stride.
+
+    With `delta` (x's shape and dtype) the residual stream moves on first: returns (x + delta, LayerNorm of
+    it), both differentiable; the sum is rounded to the dtype, and it is the rounded one that is normalised.
+    weight / bias: [columns] in x's dtype or float32 (both the same), or None for 1 / 0."""
+    _floating(x, "layer_norm")
+    if x.dim() == 0 or not 0 < x.shape[-1] <= NORM_MAX_D:
+        raise ValueError("layer_norm: 1 to %d columns, got %s" % (NORM_MAX_D, tuple(x.shape)))
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError("layer_norm: eps %r" % (eps,))
+    if delta is not None and (delta.shape != x.shape or delta.dtype != x.dtype or delta.device != x.device):
+        raise ValueError("layer_norm: delta has x's shape, dtype and device")
+    for t in (weight, bias):
+        if t is None:
+            continue
+        if t.device != x.device or t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32):
+            raise ValueError("layer_norm: weight and bias are [%d] tensors in %s or float32 on %s" % (x.shape[-1], x.dtype, x.device))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("layer_norm: weight and bias differ in dtype")
+    weight = weight if weight is None else weight.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, weight, bias)):
+        return _LayerNorm.apply(x, delta, weight, bias, eps)
+    new, h, _, _ = _norm_forward(x, delta, weight, bias, eps, False)
+    return h if new is None else (new, h)
+
+
+# ------------------------------------------------------------------------------- log probabilities
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' answer: f32 log probabilities in the tokens' shape, the rows' entropy, and the
+    `top` largest log probabilities of each row with their tokens (None where top is 0)."""
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logprobs: Optional[torch.Tensor]
+    top_tokens: Optional[torch.Tensor]
+
+
+def _logp_forward(logits, tokens, mask, temperature, top, lse):
+    lead, vocab, dev = logits.shape[:-1], logits.shape[-1], logits.device
+    xr, xs = _rows(logits)
+    rows = xr.shape[0]
+    mr, ms = (None, 0) if mask is None else (mask.contiguous(), 0) if mask.dim() == 1 and logits.dim() > 1 else _rows(mask)
+    n = 0 if tokens is None else 1 if tokens.dim() == len(lead) else tokens.shape[-1]
+    f32 = {"dtype": torch.float32, "device": dev}
+    logprobs = None if tokens is None else torch.empty(tokens.shape, **f32)
+    entropy = torch.empty(lead, **f32)
+    ls = torch.empty(lead, **f32) if lse else None
+    tl = torch.empty(lead + (top,), **f32) if top else None
+    tt = torch.empty(lead + (top,), dtype=torch.int64, device=dev) if top else None
+    L, kind = _native.lib(), _TYPES[logits.dtype]
+    size = L.dk_net_token_logprobs_workspace(rows, vocab, kind, top)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _check(_launch(L.dk_net_token_logprobs_async, dev, xr.data_ptr(), xs, rows, vocab, kind, _ptr(mr), ms, temperature,
+                   _ptr(tokens), n, top, _ptr(logprobs), entropy.data_ptr(), _ptr(ls), _ptr(tl), _ptr(tt), _ptr(ws), size),
+           "token log probabilities")
+    return logprobs, entropy, ls, tl, tt, (xr, mr, ms, n)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, temperature, top):
+        logprobs, entropy, ls, tl, tt, (xr, mr, ms, n) = _logp_forward(logits, tokens, mask, temperature, top, True)
+        ctx.save_for_backward(xr, tokens, mr, ls, entropy)
+        ctx.ms, ctx.n, ctx.temperature, ctx.shape = ms, n, temperature, logits.shape
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (tl, tt) if t is not None))
+        return logprobs, entropy, tl, tt
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogp, dent, _tl, _tt):
+        if dlogp is None and dent is None:
+            return None, None, None, None, None
+        x, tokens, mask, ls, entropy = ctx.saved_tensors
+        xr, xs = _rows(x)
+        dlogp = None if dlogp is None else dlogp.contiguous()
+        dent = None if dent is None else dent.contiguous()
+        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
+        _check(_launch(_native.lib().dk_net_token_logprobs_bwd_async, x.device, xr.data_ptr(), xs, xr.shape[0], xr.shape[1],
+                       _TYPES[x.dtype], _ptr(mask), ctx.ms, ctx.temperature, _ptr(tokens), ctx.n, ls.data_ptr(),
+                       entropy.data_ptr(), _ptr(dlogp), _ptr(dent), dx.data_ptr()), "token log probabilities backward")
+        return dx, None, None, None, None
+
+
+def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
+    """Log probabilities of given tokens under softmax(logits / temperature), with the rows' entropy and their
+    `top` (at most 32) largest alternatives; differentiable in the logits through logprobs and entropy.
+
+    logits [..., vocab]; tokens int64 or int32 [...] or [..., n] with n <= 64; a negative one is padding (log
+    probability 0, no gradient), one >= vocab gives NaN and no gradient.  mask: bool [..., vocab] or [vocab],
+    True for what is allowed; a token that is not has log probability -inf and no gradient, and what a masked
+    logit holds is not looked at.  A row with nothing allowed has entropy 0.  Alternatives are ordered by
+    logit, equal ones by index; -1 (and -inf) behind the last allowed one."""
+    _floating(logits, "token_logprobs")
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError("token_logprobs: logits need a last dimension of at least 1, got %s" % (tuple(logits.shape),))
+    lead = logits.shape[:-1]
+    if tokens is not None:
+        if tokens.device != logits.device or tokens.dtype not in (torch.int64, torch.int32):
+            raise ValueError("token_logprobs: tokens are int64 or int32 on the logits' device")
+        if tokens.shape != lead and not (tokens.dim() == len(lead) + 1 and tokens.shape[:-1] == lead and tokens.shape[-1] <= TOKENS_MAX):
+            raise ValueError("token_logprobs: tokens %s do not go with logits %s (at most %d a row)"
+                             % (tuple(tokens.shape), tuple(logits.shape), TOKENS_MAX))
+        tokens = tokens.long().contiguous()
+    if mask is not None and (mask.device != logits.device or mask.dtype != torch.bool or mask.shape not in (logits.shape, logits.shape[-1:])):
+        raise ValueError("token_logprobs: mask is bool on the logits' device, in their shape or [%d]" % logits.shape[-1])
+    temperature = float(temperature)
+    if not (temperature >= 1e-6 and math.isfinite(temperature)):
+        raise ValueError("token_logprobs: temperature %r (at least 1e-6)" % (temperature,))
+    if not 0 <= top <= TOP_MAX:
+        raise ValueError("token_logprobs: top %r (0 to %d)" % (top, TOP_MAX))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, mask, temperature, top))
+    logprobs, entropy, _, tl, tt, _ = _logp_forward(logits, tokens, mask, temperature, top, False)
+    return TokenLogprobs(logprobs, entropy, tl, tt)
+
+
+# ------------------------------------------------------------------------------- AdamW
+_ROW = np.dtype([("p", np.uint64), ("g", np.uint64), ("n", np.uint64), ("block", np.uint64), ("id", np.uint64)])
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay, bias-corrected moments) with one pass over all tensors of a group.
+
+    state_bits 32: f32 moments.  state_bits 8: e4m3 codes of exp_avg and of sqrt(exp_avg_sq) with one f32
+    scale for each 256 elements of a tensor.  master_weights: bf16 / f16 parameters are rounded copies of
+    f32 weights that the optimiser keeps; a parameter that was written to since the last step (a loaded
+    state_dict) is taken over into its master first.  lr may be a one-element f32 tensor on the GPU.
+
+    A group's parameters share one dtype and device and are dense.  The states lie in flat buffers
+    (`buffers`, one dict a group; each parameter at a multiple of 256 elements) and state[p] holds views of
+    them; `step` counts on the device for each parameter, so step() may be captured into a graph
+    (lr as a float is captured as it is)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False):
+        if state_bits not in (8, 32):
+            raise ValueError("AdamW: state_bits %r (8 or 32)" % (state_bits,))
+        self.state_bits, self.master_weights = state_bits, bool(master_weights)
+        self.buffers, self._tables = [], []
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    @torch.no_grad()
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        try:
+            self._lay_out(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def _lay_out(self, group):
+        params = group["params"]
+        _hyper(group)
+        for p in params:
+            _floating(p, "AdamW")
+            if p.dtype != params[0].dtype or p.device != params[0].device or not p.is_contiguous():
+                raise ValueError("AdamW: a group's parameters are dense and share one dtype and device")
+        master = self.master_weights and bool(params) and params[0].dtype != torch.float32
+        dev = params[0].device if params else None
+        table = np.zeros(len(params), _ROW)
+        blocks = 0
+        for i, p in enumerate(params):
+            table[i] = (0, 0, p.numel(), blocks, i)
+            blocks += -(-p.numel() // ADAMW_BLOCK)
+        b = {"step": torch.zeros(len(params), dtype=torch.int32, device=dev)}
+        for k in ("exp_avg", "exp_avg_sq"):
+            if self.state_bits == 8:
+                b[k] = torch.zeros(blocks * ADAMW_BLOCK, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+                b[k + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=dev)
+            else:
+                b[k] = torch.zeros(blocks * ADAMW_BLOCK, dtype=torch.float32, device=dev)
+        if master:
+            b["master"] = torch.zeros(blocks * ADAMW_BLOCK, dtype=torch.float32, device=dev)
+        for i, p in enumerate(params):
+            lo, n = int(table[i]["block"]), p.numel()
+            st = self.state[p] = {"step": b["step"][i]}
+            for k in b:
+                if k.endswith("_scale"):
+                    st[k] = b[k][lo:lo + -(-n // ADAMW_BLOCK)]
+                elif k != "step":
+                    st[k] = b[k][lo * ADAMW_BLOCK:lo * ADAMW_BLOCK + n].view(p.shape)
+            if master:
+                st["master"].copy_(p)
+        # (scratch of a step: the tensors' factors; and the parameters' versions that the masters go with)
+        self.buffers.append(b)
+        self._tables.append({"rows": table, "dtype": params[0].dtype if params else None, "device": dev,
+                             "factors": torch.empty(3 * max(1, len(params)), dtype=torch.float32, device=dev),
+                             "versions": [p._version for p in params] if master else None})
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group, b, t in zip(self.param_groups, self.buffers, self._tables):
+            self._step_group(group, b, t)
+        return loss
+
+    def _step_group(self, group, b, t):
+        dtype, device = t["dtype"], t["device"]
+        lr, d_lr = _hyper(group)
+        at, ps, gs, params, kept = [], [], [], [], []
+        for i, p in enumerate(group["params"]):
+            g = p.grad
+            if g is None:
+                continue
+            if p.dtype != dtype or p.device != device or not p.is_contiguous():
+                raise RuntimeError("AdamW: a parameter was moved, cast or restrided since the optimiser was made")
+            if g.dtype != dtype or g.layout != torch.strided:
+                raise ValueError("AdamW: gradients are dense and in the parameters' dtype")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                kept.append(g)
+            if t["versions"] is not None and t["versions"][i] != p._version:
+                self.state[p]["master"].copy_(p)
+            at.append(i)
+            params.append(p)
+            ps.append(p.data_ptr())
+            gs.append(g.data_ptr())
+        if not at:
+            return
+        rows = t["rows"] if len(at) == len(t["rows"]) else t["rows"][at]
+        rows["p"], rows["g"] = ps, gs
+        b1, b2 = group["betas"]
+        _check(_launch(_native.lib().dk_net_adamw_async, device, rows.ctypes.data, len(at), _TYPES[dtype], self.state_bits,
+                       b["exp_avg"].data_ptr(), b["exp_avg_sq"].data_ptr(), _ptr(b.get("exp_avg_scale")),
+                       _ptr(b.get("exp_avg_sq_scale")), _ptr(b.get("master")), b["step"].data_ptr(), t["factors"].data_ptr(),
+                       lr, _ptr(d_lr), b1, b2, group["eps"], group["weight_decay"]), "AdamW")
+        # the networks' split weights are cached by the parameters' versions
+        torch.autograd.graph.increment_version(params)
+        if t["versions"] is not None:
+            for i, p in zip(at, params):
+                t["versions"][i] = p._version
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """Takes over the states of a state_dict() of the same parameters, into the buffers that are there
+        (also torch.optim.AdamW's, where state_bits is 32)."""
+        groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("AdamW: the state_dict has other parameter groups")
+        todo = []
+        for mine, theirs in zip(self.param_groups, groups):
+            for p, key in zip(mine["params"], theirs["params"]):
+                st = state_dict["state"].get(key)
+                for k, own in self.state[p].items():
+                    if st is None or (k == "master" and k not in st):   # (not stepped yet: as at the start)
+                        todo.append((own, p if k == "master" else None))
+                        continue
+                    v = st.get(k)
+                    f8 = torch.float8_e4m3fn
+                    if not isinstance(v, torch.Tensor) or v.shape != own.shape or (own.dtype == f8) != (v.dtype == f8):
+                        raise ValueError("AdamW: the state_dict's %s does not fit (state_bits %d)" % (k, self.state_bits))
+                    todo.append((own, v))
+        for mine, theirs in zip(self.param_groups, groups):
+            mine.update({k: v for k, v in theirs.items() if k in self.defaults})
+        for own, v in todo:
+            if v is None:
+                own.view(torch.uint8 if own.dtype == torch.float8_e4m3fn else own.dtype).zero_()
+            else:
+                own.copy_(v)
+        for t, g in zip(self._tables, self.param_groups):
+            if t["versions"] is not None:
+                t["versions"] = [p._version for p in g["params"]]
+
+
+def _hyper(group):
+    """A group's learning rate as (float, device tensor or None); raises where a hyperparameter is out of range."""
+    lr, (b1, b2) = group["lr"], group["betas"]
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and group["eps"] >= 0.0 and group["weight_decay"] >= 0.0):
+        raise ValueError("AdamW: betas %r, eps %r or weight_decay %r out of range" % (group["betas"], group["eps"], group["weight_decay"]))
+    if isinstance(lr, torch.Tensor):
+        if lr.numel() != 1 or (lr.is_cuda and lr.dtype != torch.float32):
+            raise ValueError("AdamW: lr as a tensor is one float32 value")
+        return (0.0, lr) if lr.is_cuda else (float(lr), None)
+    if not lr >= 0.0:
+        raise ValueError("AdamW: lr %r" % (lr,))
+    return float(lr), None
