@@ -43,7 +43,47 @@ void with_weight(int wtype, F f) {
     else f(T{});
 }
 
-constexpr uint32_t norm_slices(uint64_t rows) { return rows >= 64u * 64u ? 64u : rows ? (uint32_t)((rows + 63u) / 64u) : 1u; }
+// calls f with the NormShape that rows of d columns of T take
+template <class T, int L, int LO, int HI, class F>
+void with_vectors(uint32_t nv, F f) {
+    if constexpr (LO == HI) f(NormShape<L, LO>{});
+    else if (nv <= (uint32_t)(L * LO)) f(NormShape<L, LO>{});
+    else with_vectors<T, L, LO + 1, HI>(nv, f);
+}
+template <class T, class F>
+void with_shape(uint32_t d, F f) {
+    constexpr int E16 = 16 / VEC<T>, E32 = 32 / VEC<T>, MORE = E16 / 2 + 1;   // vectors of 16 and of 32 elements
+    const uint32_t nv = (d + VEC<T> - 1) / VEC<T>;
+    if (nv <= 8 * E16) with_vectors<T, 8, 1, E16>(nv, f);
+    else if (nv <= 16 * E16) with_vectors<T, 16, MORE, E16>(nv, f);
+    else if (nv <= 32 * E16) with_vectors<T, 32, MORE, E16>(nv, f);
+    else if (nv <= 64 * E32) with_vectors<T, 64, MORE, E32>(nv, f);
+    else if (nv <= 256 * E16) with_vectors<T, 256, MORE, E16>(nv, f);
+    else with_vectors<T, 512, MORE, E32>(nv, f);
+}
+
+// workgroups of a norm kernel with `per` rows in a workgroup at a time
+constexpr uint32_t norm_grid(uint64_t rows, uint32_t per, uint32_t most) {
+    const uint64_t n = (rows + per - 1) / per;
+    return n == 0 ? 1u : (uint32_t)(n < most ? n : most);
+}
+constexpr uint32_t NORM_GRID = 2048;
+// The backward pass writes 2 d sums for each workgroup, as much as a row: no more workgroups than the 256 CUs
+// hold at a time by their registers (two of 256 threads: at 16384 x 4096 bf16 108 us against 129 with 1024
+// workgroups and 128 with 256; at 200000 x 160 f32 102 against 115 and 156), and at least 8 rows for each
+// beyond the first 256 (2000 x 4096 bf16: 27 us against 31 with 512).
+template <class S>
+constexpr uint32_t norm_bwd_most(uint64_t rows) { return S::THREADS > 256 || rows < 8 * 512 ? 256u : 512u; }
+uint32_t norm_bwd_grid(uint64_t rows, uint32_t d, int type) {
+    uint32_t n = 1;
+    with_type(type, [&](auto t) {
+        with_shape<decltype(t)>(d, [&](auto s) {
+            using S = decltype(s);
+            n = norm_grid(rows, S::ROWS, norm_bwd_most<S>(rows));
+        });
+    });
+    return n;
+}
 
 }  // namespace
 
@@ -57,13 +97,13 @@ int dk_net_layer_norm_async(const void* x, uint64_t x_stride, const void* delta,
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
     if (!x || !h_out) return DK_E_INVALID;
+    const NormArgs a{x, delta, x_stride, delta_stride, rows, d, wtype == DK_F32, gamma, beta, eps, 1.0f / (float)d, x_out, h_out, stats};
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        with_weight<T>(wtype, [&](auto w) {
-            using W = decltype(w);
-            hipLaunchKernelGGL((layer_norm_kernel<T, W>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream,
-                               (const T*)x, x_stride, (const T*)delta, delta_stride, rows, d, (const W*)gamma,
-                               (const W*)beta, eps, (T*)x_out, (T*)h_out, stats);
+        with_shape<T>(d, [&](auto s) {
+            using S = decltype(s);
+            hipLaunchKernelGGL((layer_norm_kernel<T, S>), dim3(norm_grid(rows, S::ROWS, NORM_GRID)), dim3(S::THREADS), 0,
+                               (hipStream_t)stream, a);
         });
     });
     DK_HIP(hipGetLastError());
@@ -71,8 +111,8 @@ int dk_net_layer_norm_async(const void* x, uint64_t x_stride, const void* delta,
 }
 
 uint64_t dk_net_layer_norm_bwd_workspace(uint64_t rows, uint32_t d, int type) {
-    (void)type;
-    return (uint64_t)norm_slices(rows) * 2 * d * sizeof(float);
+    if (!type_ok(type) || d == 0 || d > NORM_MAX_D) return 0;
+    return (uint64_t)norm_bwd_grid(rows, d, type) * 2 * d * sizeof(float);
 }
 
 int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* dx_res, uint64_t dx_res_stride, const void* x,
@@ -86,24 +126,22 @@ int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* 
     if (weights && (!workspace || workspace_bytes < dk_net_layer_norm_bwd_workspace(rows, d, type))) return DK_E_INVALID;
     if (rows == 0 && !weights) return DK_OK;
     hipStream_t st = (hipStream_t)stream;
-    const uint32_t slices = norm_slices(rows);
+    const uint32_t grid = rows ? norm_bwd_grid(rows, d, type) : 0;
+    const NormBwdArgs a{dh, dx_res, x, dh_stride, dx_res_stride, x_stride, rows, d, wtype == DK_F32, stats, gamma, 1.0f / (float)d,
+                        dx, weights ? (float*)workspace : nullptr};
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        with_weight<T>(wtype, [&](auto w) {
-            using W = decltype(w);
-            if (rows)
-                hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st,
-                                   (const T*)dh, dh_stride, (const T*)dx_res, dx_res_stride, (const T*)x, x_stride, stats,
-                                   rows, d, (const W*)gamma, (T*)dx);
-            if (weights) {
-                if (rows)
-                    hipLaunchKernelGGL(layer_norm_dw_kernel<T>, dim3((d + 63) / 64, slices), dim3(256), 0, st,
-                                       (const T*)dh, dh_stride, (const T*)x, x_stride, stats, rows, d,
-                                       (rows + slices - 1) / slices, (float*)workspace);
-                hipLaunchKernelGGL(layer_norm_dw_join_kernel<W>, dim3((2 * d + 255) / 256), dim3(256), 0, st,
-                                   (const float*)workspace, rows ? slices : 0u, d, (W*)dgamma, (W*)dbeta);
-            }
-        });
+        if (rows)
+            with_shape<T>(d, [&](auto s) {
+                using S = decltype(s);
+                hipLaunchKernelGGL((layer_norm_bwd_kernel<T, S>), dim3(grid), dim3(S::THREADS), 0, st, a);
+            });
+        if (weights)
+            with_weight<T>(wtype, [&](auto w) {
+                using W = decltype(w);
+                hipLaunchKernelGGL(layer_norm_dw_join_kernel<W>, dim3((2 * d + 15) / 16), dim3(1024), 0, st,
+                                   (const float*)workspace, grid, d, (W*)dgamma, (W*)dbeta);
+            });
     });
     DK_HIP(hipGetLastError());
     return DK_OK;

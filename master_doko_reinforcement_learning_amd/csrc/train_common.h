@@ -16,15 +16,70 @@ __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <class T>
 __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 
-// sum / maximum over the 64 lanes of a wave, in every lane; a fixed tree, so equal inputs give equal bits
-__device__ __forceinline__ float wave_sum(float v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// 16 bytes of elements.  Rows start wherever a view puts them, so the type promises no more than an
+// element's alignment: gfx950 loads and stores 16 bytes from any address in one instruction.
+template <class T>
+constexpr int VEC = 16 / (int)sizeof(T);
+template <class T>
+using Vec __attribute__((aligned(alignof(T)))) = T __attribute__((ext_vector_type(VEC<T>)));
+
+// the elements c .. c + VEC of a row of d, 0 behind its end
+template <class T>
+__device__ __forceinline__ Vec<T> load_vec(const T* row, uint32_t c, uint32_t d) {
+    if (c + VEC<T> <= d) return *(const Vec<T>*)(row + c);
+    Vec<T> v;
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j) v[j] = c + j < d ? row[c + j] : (T)0.0f;
     return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+template <class T>
+__device__ __forceinline__ void store_vec(T* row, uint32_t c, uint32_t d, Vec<T> v) {
+    if (c + VEC<T> <= d) {
+        *(Vec<T>*)(row + c) = v;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j)
+        if (c + j < d) row[c + j] = v[j];
+}
+
+// v of the lane that differs in one bit of its number (1, 2: quad permutes; 4, 8: mirrors, whose lane
+// holds the same value once the bits below are reduced; 16, 32: row swaps)
+template <int BIT>
+__device__ __forceinline__ float other(float v) {
+    const int i = __builtin_bit_cast(int, v);
+    if constexpr (BIT == 1) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0xB1, 0xF, 0xF, true));
+    else if constexpr (BIT == 2) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x4E, 0xF, 0xF, true));
+    else if constexpr (BIT == 4) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x141, 0xF, 0xF, true));
+    else return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x140, 0xF, 0xF, true));
+}
+struct Add { __device__ static float of(float a, float b) { return a + b; } };
+struct Max { __device__ static float of(float a, float b) { return fmaxf(a, b); } };
+
+// sum / maximum over groups of N lanes (a power of two up to 64), in every lane of the group; a fixed
+// tree, so equal inputs give equal bits
+template <int N, class Op>
+__device__ __forceinline__ float lanes_reduce(float v) {
+    if constexpr (N >= 2) v = Op::of(v, other<1>(v));
+    if constexpr (N >= 4) v = Op::of(v, other<2>(v));
+    if constexpr (N >= 8) v = Op::of(v, other<4>(v));
+    if constexpr (N >= 16) v = Op::of(v, other<8>(v));
+    if constexpr (N >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const uint32_t lo = s[0], hi = s[1];   // (of s[1] itself a bit cast would take s[0])
+        v = Op::of(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+    }
+    if constexpr (N >= 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const uint32_t lo = s[0], hi = s[1];   // (of s[1] itself a bit cast would take s[0])
+        v = Op::of(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+    }
     return v;
 }
+__device__ __forceinline__ float wave_sum(float v) { return lanes_reduce<64, Add>(v); }
+__device__ __forceinline__ float wave_max(float v) { return lanes_reduce<64, Max>(v); }
 
 }  // namespace train
 }  // namespace dk

@@ -23,18 +23,23 @@ def _check(rc, what):
         raise RuntimeError("doko_amd %s kernel error %d" % (what, rc))
 
 
-def _launch(fn, device, *args):
-    """fn(*args, stream) on torch's current stream of `device`, with that device current."""
-    st = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        return fn(*args, st)
-    with torch.cuda.device(device):
-        return fn(*args, st)
+# torch's current stream of a device as an integer (the public call makes a Stream object each time, 2 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _launch(fn, index, *args):
+    """fn(*args, stream) on torch's current stream of device `index`, with that device current."""
+    if index == torch.cuda.current_device():
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
 
 def _rows(t):
-    """t as rows over its last dimension: (2-D tensor with a dense last dimension, elements between rows).
+    """t as rows over its last dimension: (a tensor with that memory, elements between rows).
     Copies only what has no such view."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     r = t.reshape(-1, t.shape[-1])
     if r.stride(1) != 1 and r.shape[1] > 1:
         r = r.contiguous()
@@ -54,53 +59,65 @@ def _ptr(t):
 
 
 # ------------------------------------------------------------------------------- layer norm
+def _dense_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _norm_forward(x, delta, weight, bias, eps, stats):
     d = x.shape[-1]
+    rows = x.numel() // d
     xr, xs = _rows(x)
     dr, ds = _rows(delta) if delta is not None else (None, 0)
-    rows = xr.shape[0]
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    new = torch.empty(x.shape, dtype=x.dtype, device=x.device) if delta is not None else None
-    st = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if stats else None
+    h = _dense_like(x)
+    new = _dense_like(x) if delta is not None else None
+    st = x.new_empty((rows, 2), dtype=torch.float32) if stats else None
     w = weight if weight is not None else bias
-    _check(_launch(_native.lib().dk_net_layer_norm_async, x.device, xr.data_ptr(), xs, _ptr(dr), ds, rows, d, _TYPES[x.dtype],
+    _check(_launch(_native.lib().dk_net_layer_norm_async, x.get_device(), xr.data_ptr(), xs, _ptr(dr), ds, rows, d, _TYPES[x.dtype],
                    _ptr(weight), _ptr(bias), _TYPES[w.dtype] if w is not None else 0, eps, _ptr(new), h.data_ptr(), _ptr(st)),
            "layer norm")
     return new, h, st, xr
+
+
+def _norm_backward(ctx, *grads):
+    dres, dh = (None, grads[0]) if len(grads) == 1 else grads
+    need_x, need_delta, need_w, need_b, _ = ctx.needs_input_grad
+    if dh is None:
+        return (dres if need_x else None), (dres if need_delta else None), None, None, None
+    x, st, weight = ctx.saved_tensors
+    wdtype = weight.dtype if weight is not None else ctx.wdtype
+    rows, d, kind = st.shape[0], x.shape[-1], _TYPES[x.dtype]
+    xr, xs = _rows(x)
+    gr, gs = _rows(dh)
+    rr, rs = _rows(dres) if dres is not None else (None, 0)
+    dx = _dense_like(x)
+    dw = x.new_empty(d, dtype=wdtype) if need_w else None
+    db = x.new_empty(d, dtype=wdtype) if need_b else None
+    L = _native.lib()
+    size = L.dk_net_layer_norm_bwd_workspace(rows, d, kind) if need_w or need_b else 0
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
+    _check(_launch(L.dk_net_layer_norm_bwd_async, x.get_device(), gr.data_ptr(), gs, _ptr(rr), rs, xr.data_ptr(), xs, st.data_ptr(),
+                   rows, d, kind, _ptr(weight), _TYPES[wdtype], dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), size),
+           "layer norm backward")
+    if dx.shape != ctx.shape:   # (x was copied into rows)
+        dx = dx.view(ctx.shape)
+    return (dx if need_x else None), (dx if need_delta else None), dw, db, None
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, weight, bias, eps):
         new, h, st, xr = _norm_forward(x, delta, weight, bias, eps, True)
-        ctx.shape, ctx.bias = x.shape, None if bias is None else bias.dtype
-        ctx.save_for_backward(new if new is not None else xr, st, weight)
+        ctx.shape, ctx.wdtype = x.shape, torch.float32 if bias is None else bias.dtype
+        ctx.save_for_backward(xr if new is None else new, st, weight)
         ctx.set_materialize_grads(False)
         return h if new is None else (new, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        dres, dh = (None, grads[0]) if len(grads) == 1 else grads
-        need_x, need_delta, need_w, need_b = ctx.needs_input_grad[:4]
-        if dh is None:
-            return (dres if need_x else None), (dres if need_delta else None), None, None, None
-        x, st, weight = ctx.saved_tensors
-        xr, xs = _rows(x)
-        rows, d = xr.shape
-        gr, gs = _rows(dh)
-        rr, rs = _rows(dres) if dres is not None else (None, 0)
-        wdtype = weight.dtype if weight is not None else ctx.bias if ctx.bias is not None else torch.float32
-        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty(d, dtype=wdtype, device=x.device) if need_w else None
-        db = torch.empty(d, dtype=wdtype, device=x.device) if need_b else None
-        L = _native.lib()
-        size = L.dk_net_layer_norm_bwd_workspace(rows, d, _TYPES[x.dtype]) if need_w or need_b else 0
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        _check(_launch(L.dk_net_layer_norm_bwd_async, x.device, gr.data_ptr(), gs, _ptr(rr), rs, xr.data_ptr(), xs, st.data_ptr(),
-                       rows, d, _TYPES[x.dtype], _ptr(weight), _TYPES[wdtype], dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), size),
-               "layer norm backward")
-        return (dx if need_x else None), (dx if need_delta else None), dw, db, None
+    def backward(ctx, *grads):   # (the check against a second derivative only where one is asked for: 4 us)
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, *grads)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, delta=None):
@@ -142,24 +159,41 @@ class TokenLogprobs(NamedTuple):
 
 
 def _logp_forward(logits, tokens, mask, temperature, top, lse):
-    lead, vocab, dev = logits.shape[:-1], logits.shape[-1], logits.device
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    rows = logits.numel() // vocab
     xr, xs = _rows(logits)
-    rows = xr.shape[0]
     mr, ms = (None, 0) if mask is None else (mask.contiguous(), 0) if mask.dim() == 1 and logits.dim() > 1 else _rows(mask)
     n = 0 if tokens is None else 1 if tokens.dim() == len(lead) else tokens.shape[-1]
-    f32 = {"dtype": torch.float32, "device": dev}
-    logprobs = None if tokens is None else torch.empty(tokens.shape, **f32)
-    entropy = torch.empty(lead, **f32)
-    ls = torch.empty(lead, **f32) if lse else None
-    tl = torch.empty(lead + (top,), **f32) if top else None
-    tt = torch.empty(lead + (top,), dtype=torch.int64, device=dev) if top else None
+    f32 = torch.float32
+    logprobs = None if tokens is None else logits.new_empty(tokens.shape, dtype=f32)
+    entropy = logits.new_empty(lead, dtype=f32)
+    ls = logits.new_empty(lead, dtype=f32) if lse else None
+    tl = logits.new_empty(lead + (top,), dtype=f32) if top else None
+    tt = logits.new_empty(lead + (top,), dtype=torch.int64) if top else None
     L, kind = _native.lib(), _TYPES[logits.dtype]
     size = L.dk_net_token_logprobs_workspace(rows, vocab, kind, top)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    _check(_launch(L.dk_net_token_logprobs_async, dev, xr.data_ptr(), xs, rows, vocab, kind, _ptr(mr), ms, temperature,
+    ws = logits.new_empty(size, dtype=torch.uint8) if size else None
+    _check(_launch(L.dk_net_token_logprobs_async, logits.get_device(), xr.data_ptr(), xs, rows, vocab, kind, _ptr(mr), ms, temperature,
                    _ptr(tokens), n, top, _ptr(logprobs), entropy.data_ptr(), _ptr(ls), _ptr(tl), _ptr(tt), _ptr(ws), size),
            "token log probabilities")
     return logprobs, entropy, ls, tl, tt, (xr, mr, ms, n)
+
+
+def _logp_backward(ctx, dlogp, dent, _tl, _tt):
+    if dlogp is None and dent is None:
+        return None, None, None, None, None
+    x, tokens, mask, ls, entropy = ctx.saved_tensors
+    xr, xs = _rows(x)
+    dlogp = None if dlogp is None else dlogp.contiguous()
+    dent = None if dent is None else dent.contiguous()
+    dx = x.new_empty(ctx.shape)
+    _check(_launch(_native.lib().dk_net_token_logprobs_bwd_async, x.get_device(), xr.data_ptr(), xs, ls.numel(), x.shape[-1],
+                   _TYPES[x.dtype], _ptr(mask), ctx.ms, ctx.temperature, _ptr(tokens), ctx.n, ls.data_ptr(),
+                   entropy.data_ptr(), _ptr(dlogp), _ptr(dent), dx.data_ptr()), "token log probabilities backward")
+    return dx, None, None, None, None
+
+
+_logp_backward_once = torch.autograd.function.once_differentiable(_logp_backward)
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -169,23 +203,13 @@ class _TokenLogprobs(torch.autograd.Function):
         ctx.save_for_backward(xr, tokens, mr, ls, entropy)
         ctx.ms, ctx.n, ctx.temperature, ctx.shape = ms, n, temperature, logits.shape
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (tl, tt) if t is not None))
+        if top:
+            ctx.mark_non_differentiable(tl, tt)
         return logprobs, entropy, tl, tt
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dlogp, dent, _tl, _tt):
-        if dlogp is None and dent is None:
-            return None, None, None, None, None
-        x, tokens, mask, ls, entropy = ctx.saved_tensors
-        xr, xs = _rows(x)
-        dlogp = None if dlogp is None else dlogp.contiguous()
-        dent = None if dent is None else dent.contiguous()
-        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
-        _check(_launch(_native.lib().dk_net_token_logprobs_bwd_async, x.device, xr.data_ptr(), xs, xr.shape[0], xr.shape[1],
-                       _TYPES[x.dtype], _ptr(mask), ctx.ms, ctx.temperature, _ptr(tokens), ctx.n, ls.data_ptr(),
-                       entropy.data_ptr(), _ptr(dlogp), _ptr(dent), dx.data_ptr()), "token log probabilities backward")
-        return dx, None, None, None, None
+    def backward(ctx, *grads):
+        return (_logp_backward_once if torch.is_grad_enabled() else _logp_backward)(ctx, *grads)
 
 
 def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
@@ -329,7 +353,7 @@ class AdamW(torch.optim.Optimizer):
         rows = t["rows"] if len(at) == len(t["rows"]) else t["rows"][at]
         rows["p"], rows["g"] = ps, gs
         b1, b2 = group["betas"]
-        _check(_launch(_native.lib().dk_net_adamw_async, device, rows.ctypes.data, len(at), _TYPES[dtype], self.state_bits,
+        _check(_launch(_native.lib().dk_net_adamw_async, device.index, rows.ctypes.data, len(at), _TYPES[dtype], self.state_bits,
                        b["exp_avg"].data_ptr(), b["exp_avg_sq"].data_ptr(), _ptr(b.get("exp_avg_scale")),
                        _ptr(b.get("exp_avg_sq_scale")), _ptr(b.get("master")), b["step"].data_ptr(), t["factors"].data_ptr(),
                        lr, _ptr(d_lr), b1, b2, group["eps"], group["weight_decay"]), "AdamW")
