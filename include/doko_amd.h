@@ -655,27 +655,27 @@ int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* 
  *   logprobs [rows][n]    z[tokens[i]] - log sum e^z; 0 for a negative token (padding), -inf for one that is
  *                         not allowed or holds -inf, NaN for one >= vocab (nothing is read there)
  *   entropy [rows]        of the row's distribution (NULL: not wanted)
- *   lse [rows]            log sum e^z, for the backward pass (NULL: not wanted)
+ *   stats [rows][2]       the largest allowed logit and log sum e^(z - its z), for the backward pass (NULL: not wanted)
  *   top_logprobs, top_tokens [rows][top]   the largest by (logit descending, index ascending); where fewer are
  *                         allowed -inf and -1
- * n <= 64, top <= 32.  A row with nothing allowed has entropy 0 and lse -inf.  Whatever a masked entry
+ * n <= 64, top <= 32.  A row with nothing allowed has entropy 0.  Whatever a masked entry
  * holds is not looked at; a NaN or +inf in an allowed one makes the row's floating results NaN (its
  * top_tokens are still tokens of the row, NaN never among them).
  * mask_stride 0 applies one mask to every row.  The workspace has dk_net_token_logprobs_workspace bytes
  * (which may be 0: then it may be NULL).
  * dk_net_token_logprobs_bwd_async: dlogits (dense [rows][vocab], of `type`, not the logits' own buffer)
- * from dlogprobs [rows][n] and dentropy [rows] (either may be NULL), with lse and entropy of the
+ * from dlogprobs [rows][n] and dentropy [rows] (either may be NULL), with logprobs, stats and entropy of the
  * forward call.  A token given twice takes both gradients; padding, out-of-range and
  * disallowed tokens take none, nor do disallowed entries. */
 int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t rows, uint32_t vocab, int type,
                                 const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
-                                uint32_t n, uint32_t top, float* logprobs, float* entropy, float* lse, float* top_logprobs,
+                                uint32_t n, uint32_t top, float* logprobs, float* entropy, float* stats, float* top_logprobs,
                                 int64_t* top_tokens, void* workspace, uint64_t workspace_bytes, void* stream);
 uint64_t dk_net_token_logprobs_workspace(uint64_t rows, uint32_t vocab, int type, uint32_t top);
 int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_t rows, uint32_t vocab, int type,
                                     const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
-                                    uint32_t n, const float* lse, const float* entropy, const float* dlogprobs,
-                                    const float* dentropy, void* dlogits, void* stream);
+                                    uint32_t n, const float* logprobs, const float* stats, const float* entropy,
+                                    const float* dlogprobs, const float* dentropy, void* dlogits, void* stream);
 
 /* dk_net_adamw_async: one AdamW step of `count` tensors (host array; dense parameters and gradients of
  * `type`).  A tensor's states are the blocks of 256 elements from `block` on in the flat buffers; no block

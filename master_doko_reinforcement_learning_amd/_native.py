@@ -157,7 +157,7 @@ def lib():
                                                        vp, vp, vp, vp, vp, u64, vp]),
         "dk_net_token_logprobs_workspace": (u64, [u64, u32, ctypes.c_int, u32]),
         "dk_net_token_logprobs_bwd_async": (ctypes.c_int, [vp, u64, u64, u32, ctypes.c_int, vp, u64, ctypes.c_float, vp, u32, vp, vp,
-                                                           vp, vp, vp, vp]),
+                                                           vp, vp, vp, vp, vp]),
         "dk_net_adamw_async": (ctypes.c_int, [vp, u32, ctypes.c_int, ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, ctypes.c_double, vp,
                                               ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, vp]),
     }

@@ -85,6 +85,35 @@ uint32_t norm_bwd_grid(uint64_t rows, uint32_t d, int type) {
     return n;
 }
 
+// Calls f with the lanes of a row and the elements of each, as types, for vocabularies up to LOGP_SMALL:
+// 16 lanes up to 64 entries (the networks' 33 and 39 classes), a wave up to 1024.
+constexpr uint32_t LOGP_SMALL = 1024;
+template <int G_, int E_>
+struct LogpShape { static constexpr int G = G_, E = E_; };
+template <class F>
+void with_small_vocab(uint32_t vocab, F f) {
+    if (vocab <= 16) f(LogpShape<16, 1>{});
+    else if (vocab <= 32) f(LogpShape<16, 2>{});
+    else if (vocab <= 48) f(LogpShape<16, 3>{});
+    else if (vocab <= 64) f(LogpShape<16, 4>{});
+    else if (vocab <= 128) f(LogpShape<64, 2>{});
+    else if (vocab <= 256) f(LogpShape<64, 4>{});
+    else if (vocab <= 512) f(LogpShape<64, 8>{});
+    else f(LogpShape<64, 16>{});
+}
+// Workgroups that share a row: rows alone where they fill the GPU, otherwise parts of at least 2 vectors a thread.
+constexpr uint32_t LOGP_FILL = 1024, LOGP_GRID = 1u << 20;
+struct LogpSplit { uint32_t splits, elems; };
+LogpSplit logp_split(uint64_t rows, uint32_t vocab, int type) {
+    const uint32_t unit = 256u * (type == DK_F32 ? 4u : 8u);   // a vector a thread
+    const uint32_t units = (vocab + unit - 1) / unit;
+    const uint64_t want = rows >= LOGP_FILL ? 1 : LOGP_FILL / (rows ? rows : 1);
+    const uint32_t each = want >= units ? 2u : (uint32_t)((units + want - 1) / want);
+    const uint32_t splits = (units + (each < 2 ? 2 : each) - 1) / (each < 2 ? 2 : each);
+    return {splits, (each < 2 ? 2 : each) * unit};
+}
+uint32_t logp_grid(uint64_t jobs) { return (uint32_t)(jobs < LOGP_GRID ? jobs : LOGP_GRID); }
+
 }  // namespace
 
 extern "C" {
@@ -149,42 +178,68 @@ int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* 
 
 int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t rows, uint32_t vocab, int type,
                                 const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
-                                uint32_t n, uint32_t top, float* logprobs, float* entropy, float* lse, float* top_logprobs,
+                                uint32_t n, uint32_t top, float* logprobs, float* entropy, float* stats, float* top_logprobs,
                                 int64_t* top_tokens, void* workspace, uint64_t workspace_bytes, void* stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || top > TOP_MAX || rows > MAX_GRID ||
         !(temperature > 0.0f) || std::isinf(temperature))
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
     if (!logits || (n && (!tokens || !logprobs)) || (top && (!top_logprobs || !top_tokens))) return DK_E_INVALID;
+    const uint64_t need = dk_net_token_logprobs_workspace(rows, vocab, type, top);
+    if (need && (!workspace || workspace_bytes < need)) return DK_E_INVALID;
+    const LogpSplit split = logp_split(rows, vocab, type);
+    float* part = (float*)workspace;
     const LogpArgs a{logits, stride, rows, vocab, n, top, mask, mask_stride, 1.0f / temperature, tokens, logprobs, entropy,
-                     lse, top_logprobs, top_tokens};
+                     stats, top_logprobs, top_tokens, split.splits, split.elems, part,
+                     (uint64_t*)(part + 4 * rows * split.splits)};
+    hipStream_t st = (hipStream_t)stream;
     with_type(type, [&](auto t) {
-        hipLaunchKernelGGL(token_logprobs_kernel<decltype(t)>, dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);
+        using T = decltype(t);
+        if (vocab <= LOGP_SMALL) {
+            with_small_vocab(vocab, [&](auto s) {
+                using S = decltype(s);
+                hipLaunchKernelGGL((token_logprobs_small_kernel<T, S::G, S::E>), dim3(logp_grid((rows * S::G + 255) / 256)),
+                                   dim3(256), 0, st, a);
+            });
+            return;
+        }
+        hipLaunchKernelGGL(token_logprobs_kernel<T>, dim3(logp_grid(rows * split.splits)), dim3(256), 0, st, a);
+        if (split.splits > 1) hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3((uint32_t)rows), dim3(256), 0, st, a);
     });
     DK_HIP(hipGetLastError());
     return DK_OK;
 }
 
+// (a row's parts: maximum, S and U of each, then their top entries; none where a workgroup takes a row)
 uint64_t dk_net_token_logprobs_workspace(uint64_t rows, uint32_t vocab, int type, uint32_t top) {
-    (void)rows; (void)vocab; (void)type; (void)top;
-    return 0;
+    if (!type_ok(type) || rows == 0 || vocab <= LOGP_SMALL) return 0;
+    const uint32_t splits = logp_split(rows, vocab, type).splits;
+    return splits > 1 ? rows * splits * (4 * sizeof(float) + top * sizeof(uint64_t)) : 0;
 }
 
 int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_t rows, uint32_t vocab, int type,
                                     const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
-                                    uint32_t n, const float* lse, const float* entropy, const float* dlogprobs,
-                                    const float* dentropy, void* dlogits, void* stream) {
+                                    uint32_t n, const float* logprobs, const float* stats, const float* entropy,
+                                    const float* dlogprobs, const float* dentropy, void* dlogits, void* stream) {
     if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || rows > MAX_GRID || !(temperature > 0.0f) ||
         std::isinf(temperature))
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
-    if (!logits || (n && !tokens) || !lse || !entropy || !dlogits) return DK_E_INVALID;
-    const LogpBwdArgs a{logits, stride, rows, vocab, n, mask, mask_stride, 1.0f / temperature, tokens, lse, entropy,
-                        dlogprobs, dentropy, dlogits};
+    if (!logits || (n && (!tokens || !logprobs)) || !stats || !entropy || !dlogits) return DK_E_INVALID;
+    const uint32_t unit = 256u * 4u * (type == DK_F32 ? 4u : 8u), parts = (vocab + unit - 1) / unit;
+    const LogpBwdArgs a{logits, stride, rows, vocab, n, mask, mask_stride, 1.0f / temperature, tokens, logprobs, stats, entropy,
+                        dlogprobs, dentropy, dlogits, parts};
+    hipStream_t st = (hipStream_t)stream;
     with_type(type, [&](auto t) {
-        hipLaunchKernelGGL(token_logprobs_bwd_kernel<decltype(t)>, dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);
+        using T = decltype(t);
+        if (vocab <= LOGP_SMALL)
+            with_small_vocab(vocab, [&](auto s) {
+                using S = decltype(s);
+                hipLaunchKernelGGL((token_logprobs_small_bwd_kernel<T, S::G, S::E>), dim3(logp_grid((rows * S::G + 255) / 256)),
+                                   dim3(256), 0, st, a);
+            });
+        else
+            hipLaunchKernelGGL(token_logprobs_bwd_kernel<T>, dim3(logp_grid(rows * parts)), dim3(256), 0, st, a);
     });
     DK_HIP(hipGetLastError());
     return DK_OK;

@@ -44,37 +44,38 @@ __device__ __forceinline__ void store_vec(T* row, uint32_t c, uint32_t d, Vec<T>
 }
 
 // v of the lane that differs in one bit of its number (1, 2: quad permutes; 4, 8: mirrors, whose lane
-// holds the same value once the bits below are reduced; 16, 32: row swaps)
-template <int BIT>
-__device__ __forceinline__ float other(float v) {
-    const int i = __builtin_bit_cast(int, v);
-    if constexpr (BIT == 1) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0xB1, 0xF, 0xF, true));
-    else if constexpr (BIT == 2) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x4E, 0xF, 0xF, true));
-    else if constexpr (BIT == 4) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x141, 0xF, 0xF, true));
-    else return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x140, 0xF, 0xF, true));
+// holds the same value once the bits below are reduced)
+template <int BIT, class U>
+__device__ __forceinline__ U other(U v) {
+    constexpr int CTRL = BIT == 1 ? 0xB1 : BIT == 2 ? 0x4E : BIT == 4 ? 0x141 : 0x140;
+    return __builtin_bit_cast(U, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
 struct Add { __device__ static float of(float a, float b) { return a + b; } };
-struct Max { __device__ static float of(float a, float b) { return fmaxf(a, b); } };
+struct Max {
+    __device__ static float of(float a, float b) { return fmaxf(a, b); }
+    __device__ static uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; }
+};
+struct Min { __device__ static uint32_t of(uint32_t a, uint32_t b) { return a < b ? a : b; } };
 
-// sum / maximum over groups of N lanes (a power of two up to 64), in every lane of the group; a fixed
-// tree, so equal inputs give equal bits
-template <int N, class Op>
-__device__ __forceinline__ float lanes_reduce(float v) {
+// sum / maximum / minimum over groups of N lanes (a power of two up to 64), in every lane of the group;
+// a fixed tree, so equal inputs give equal bits.  U: float or uint32_t.
+template <int N, class Op, class U>
+__device__ __forceinline__ U lanes_reduce(U v) {
     if constexpr (N >= 2) v = Op::of(v, other<1>(v));
     if constexpr (N >= 4) v = Op::of(v, other<2>(v));
     if constexpr (N >= 8) v = Op::of(v, other<4>(v));
     if constexpr (N >= 16) v = Op::of(v, other<8>(v));
-    if constexpr (N >= 32) {
+    if constexpr (N >= 32) {   // (rows of 16, then halves, exchanged between two copies)
         const uint32_t u = __builtin_bit_cast(uint32_t, v);
         const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
         const uint32_t lo = s[0], hi = s[1];   // (of s[1] itself a bit cast would take s[0])
-        v = Op::of(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+        v = Op::of(__builtin_bit_cast(U, lo), __builtin_bit_cast(U, hi));
     }
     if constexpr (N >= 64) {
         const uint32_t u = __builtin_bit_cast(uint32_t, v);
         const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-        const uint32_t lo = s[0], hi = s[1];   // (of s[1] itself a bit cast would take s[0])
-        v = Op::of(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+        const uint32_t lo = s[0], hi = s[1];
+        v = Op::of(__builtin_bit_cast(U, lo), __builtin_bit_cast(U, hi));
     }
     return v;
 }

@@ -158,7 +158,7 @@ class TokenLogprobs(NamedTuple):
     top_tokens: Optional[torch.Tensor]
 
 
-def _logp_forward(logits, tokens, mask, temperature, top, lse):
+def _logp_forward(logits, tokens, mask, temperature, top, stats):
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     rows = logits.numel() // vocab
     xr, xs = _rows(logits)
@@ -167,28 +167,28 @@ def _logp_forward(logits, tokens, mask, temperature, top, lse):
     f32 = torch.float32
     logprobs = None if tokens is None else logits.new_empty(tokens.shape, dtype=f32)
     entropy = logits.new_empty(lead, dtype=f32)
-    ls = logits.new_empty(lead, dtype=f32) if lse else None
+    st = logits.new_empty((rows, 2), dtype=f32) if stats else None
     tl = logits.new_empty(lead + (top,), dtype=f32) if top else None
     tt = logits.new_empty(lead + (top,), dtype=torch.int64) if top else None
     L, kind = _native.lib(), _TYPES[logits.dtype]
     size = L.dk_net_token_logprobs_workspace(rows, vocab, kind, top)
     ws = logits.new_empty(size, dtype=torch.uint8) if size else None
     _check(_launch(L.dk_net_token_logprobs_async, logits.get_device(), xr.data_ptr(), xs, rows, vocab, kind, _ptr(mr), ms, temperature,
-                   _ptr(tokens), n, top, _ptr(logprobs), entropy.data_ptr(), _ptr(ls), _ptr(tl), _ptr(tt), _ptr(ws), size),
+                   _ptr(tokens), n, top, _ptr(logprobs), entropy.data_ptr(), _ptr(st), _ptr(tl), _ptr(tt), _ptr(ws), size),
            "token log probabilities")
-    return logprobs, entropy, ls, tl, tt, (xr, mr, ms, n)
+    return logprobs, entropy, st, tl, tt, (xr, mr, ms, n)
 
 
 def _logp_backward(ctx, dlogp, dent, _tl, _tt):
     if dlogp is None and dent is None:
         return None, None, None, None, None
-    x, tokens, mask, ls, entropy = ctx.saved_tensors
+    x, tokens, mask, logprobs, st, entropy = ctx.saved_tensors
     xr, xs = _rows(x)
     dlogp = None if dlogp is None else dlogp.contiguous()
     dent = None if dent is None else dent.contiguous()
     dx = x.new_empty(ctx.shape)
-    _check(_launch(_native.lib().dk_net_token_logprobs_bwd_async, x.get_device(), xr.data_ptr(), xs, ls.numel(), x.shape[-1],
-                   _TYPES[x.dtype], _ptr(mask), ctx.ms, ctx.temperature, _ptr(tokens), ctx.n, ls.data_ptr(),
+    _check(_launch(_native.lib().dk_net_token_logprobs_bwd_async, x.get_device(), xr.data_ptr(), xs, st.shape[0], x.shape[-1],
+                   _TYPES[x.dtype], _ptr(mask), ctx.ms, ctx.temperature, _ptr(tokens), ctx.n, _ptr(logprobs), st.data_ptr(),
                    entropy.data_ptr(), _ptr(dlogp), _ptr(dent), dx.data_ptr()), "token log probabilities backward")
     return dx, None, None, None, None
 
@@ -199,8 +199,8 @@ _logp_backward_once = torch.autograd.function.once_differentiable(_logp_backward
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, mask, temperature, top):
-        logprobs, entropy, ls, tl, tt, (xr, mr, ms, n) = _logp_forward(logits, tokens, mask, temperature, top, True)
-        ctx.save_for_backward(xr, tokens, mr, ls, entropy)
+        logprobs, entropy, st, tl, tt, (xr, mr, ms, n) = _logp_forward(logits, tokens, mask, temperature, top, True)
+        ctx.save_for_backward(xr, tokens, mr, logprobs, st, entropy)
         ctx.ms, ctx.n, ctx.temperature, ctx.shape = ms, n, temperature, logits.shape
         ctx.set_materialize_grads(False)
         if top:
