@@ -25,7 +25,8 @@ using namespace dk::train;
     } while (0)
 
 constexpr uint32_t NORM_MAX_D = 16384;
-constexpr uint64_t MAX_GRID = 0x7FFFFFFFull;
+constexpr uint64_t MAX_ROWS = 0x7FFFFFFFull;
+constexpr uint64_t ADAMW_GRID = 1ull << 23;   // workgroups of a launch: 2^33 elements
 
 bool type_ok(int t) { return t == DK_F32 || t == DK_BF16 || t == DK_F16; }
 
@@ -122,7 +123,7 @@ int dk_net_layer_norm_async(const void* x, uint64_t x_stride, const void* delta,
                             uint32_t d, int type, const void* gamma, const void* beta, int wtype, float eps, void* x_out,
                             void* h_out, float* stats, void* stream) {
     if (!type_ok(type) || (wtype != DK_F32 && wtype != type) || d == 0 || d > NORM_MAX_D || (delta && !x_out) ||
-        rows > MAX_GRID)
+        rows > MAX_ROWS)
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
     if (!x || !h_out) return DK_E_INVALID;
@@ -148,7 +149,7 @@ int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* 
                                 uint64_t x_stride, const float* stats, uint64_t rows, uint32_t d, int type,
                                 const void* gamma, int wtype, void* dx, void* dgamma, void* dbeta, void* workspace,
                                 uint64_t workspace_bytes, void* stream) {
-    if (!type_ok(type) || (wtype != DK_F32 && wtype != type) || d == 0 || d > NORM_MAX_D || rows > MAX_GRID)
+    if (!type_ok(type) || (wtype != DK_F32 && wtype != type) || d == 0 || d > NORM_MAX_D || rows > MAX_ROWS)
         return DK_E_INVALID;
     if (rows && (!dh || !x || !stats || !dx)) return DK_E_INVALID;
     const bool weights = dgamma || dbeta;
@@ -180,7 +181,7 @@ int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t ro
                                 const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
                                 uint32_t n, uint32_t top, float* logprobs, float* entropy, float* stats, float* top_logprobs,
                                 int64_t* top_tokens, void* workspace, uint64_t workspace_bytes, void* stream) {
-    if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || top > TOP_MAX || rows > MAX_GRID ||
+    if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || top > TOP_MAX || rows > MAX_ROWS ||
         !(temperature > 0.0f) || std::isinf(temperature))
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
@@ -221,7 +222,7 @@ int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_
                                     const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
                                     uint32_t n, const float* logprobs, const float* stats, const float* entropy,
                                     const float* dlogprobs, const float* dentropy, void* dlogits, void* stream) {
-    if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || rows > MAX_GRID || !(temperature > 0.0f) ||
+    if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || rows > MAX_ROWS || !(temperature > 0.0f) ||
         std::isinf(temperature))
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
@@ -256,10 +257,19 @@ int dk_net_adamw_async(const dk_net_adamw_tensor* tensors, uint32_t count, int t
     if (!tensors || !exp_avg || !exp_avg_sq || !step || !factors || (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)))
         return DK_E_INVALID;
     for (uint32_t i = 0; i < count; ++i)
-        if ((tensors[i].n && (!tensors[i].p || !tensors[i].g)) || tensors[i].n > MAX_GRID * ADAMW_BLOCK) return DK_E_INVALID;
+        if ((tensors[i].n && (!tensors[i].p || !tensors[i].g)) || tensors[i].n > ADAMW_GRID * 4 * ADAMW_BLOCK ||
+            tensors[i].block > 0xFFFFFFFFull || tensors[i].id > 0xFFFFFFFFull)
+            return DK_E_INVALID;
     const AdamwArgs a{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, exp_avg, exp_avg_sq,
                       exp_avg_scale, exp_avg_sq_scale, master, factors};
     hipStream_t st = (hipStream_t)stream;
+    AdamwTicks tick;
+    for (uint32_t at = 0; at < count; at += tick.count) {
+        tick.count = count - at < ADAMW_TICKS ? count - at : ADAMW_TICKS;
+        for (uint32_t i = 0; i < tick.count; ++i) tick.id[i] = (uint32_t)tensors[at + i].id;
+        hipLaunchKernelGGL(adamw_tick_kernel, dim3((tick.count + 63) / 64), dim3(64), 0, st, tick, lr, d_lr, std::log(beta1),
+                           std::log(beta2), weight_decay, step, factors);
+    }
     AdamwTable tab;
     for (uint32_t at = 0; at < count;) {
         uint32_t k = 0;
@@ -267,25 +277,22 @@ int dk_net_adamw_async(const dk_net_adamw_tensor* tensors, uint32_t count, int t
         for (; k < ADAMW_TENSORS && at < count; ++k, ++at) {
             const dk_net_adamw_tensor& t = tensors[at];
             const uint64_t more = (t.n + 4 * ADAMW_BLOCK - 1) / (4 * ADAMW_BLOCK);
-            if (groups + more > MAX_GRID) break;
-            tab.p[k] = t.p; tab.g[k] = t.g; tab.n[k] = t.n; tab.block[k] = t.block; tab.id[k] = t.id;
+            if (k && groups + more > ADAMW_GRID) break;
+            tab.p[k] = t.p; tab.g[k] = t.g; tab.n[k] = t.n; tab.block[k] = (uint32_t)t.block; tab.id[k] = (uint32_t)t.id;
             tab.first[k] = (uint32_t)groups;
             groups += more;
         }
         tab.count = k;
-        tab.first[k] = (uint32_t)groups;
-        hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(ADAMW_TENSORS), 0, st, tab, lr, d_lr, std::log(beta1),
-                           std::log(beta2), weight_decay, step, factors);
-        if (groups)
-            with_type(type, [&](auto t) {
-                using T = decltype(t);
-                if (state_bits == 8)
-                    hipLaunchKernelGGL((adamw_kernel<T, 8>), dim3((uint32_t)groups), dim3(256), 0, st, tab, a);
-                else
-                    hipLaunchKernelGGL((adamw_kernel<T, 32>), dim3((uint32_t)groups), dim3(256), 0, st, tab, a);
-            });
-        DK_HIP(hipGetLastError());
+        if (groups == 0) continue;
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            if (state_bits == 8)
+                hipLaunchKernelGGL((adamw_kernel<T, 8>), dim3((uint32_t)groups), dim3(256), 0, st, tab, a);
+            else
+                hipLaunchKernelGGL((adamw_kernel<T, 32>), dim3((uint32_t)groups), dim3(256), 0, st, tab, a);
+        });
     }
+    DK_HIP(hipGetLastError());
     return DK_OK;
 }
 

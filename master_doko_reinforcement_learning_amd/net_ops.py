@@ -6,7 +6,9 @@ dk_net_adamw_async; csrc/train_*_kernels.h) on torch's current stream of the ten
 first two are differentiable (once).  f32, bf16 and f16; sums and statistics are f32.  There is no CPU
 fallback.  DokoAzNet.loss / DokoImpiNet.loss are built on the first two, NetTrainer on all three.
 """
+import itertools
 import math
+import operator
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -246,6 +248,8 @@ def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
 
 
 # ------------------------------------------------------------------------------- AdamW
+_GRAD, _DTYPE, _DEVICE, _LAYOUT = (operator.attrgetter(k) for k in ("grad", "dtype", "device", "layout"))
+_DENSE, _PTR = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 _ROW = np.dtype([("p", np.uint64), ("g", np.uint64), ("n", np.uint64), ("block", np.uint64), ("id", np.uint64)])
 
 
@@ -330,38 +334,39 @@ class AdamW(torch.optim.Optimizer):
     def _step_group(self, group, b, t):
         dtype, device = t["dtype"], t["device"]
         lr, d_lr = _hyper(group)
-        at, ps, gs, params, kept = [], [], [], [], []
-        for i, p in enumerate(group["params"]):
-            g = p.grad
-            if g is None:
-                continue
-            if p.dtype != dtype or p.device != device or not p.is_contiguous():
-                raise RuntimeError("AdamW: a parameter was moved, cast or restrided since the optimiser was made")
-            if g.dtype != dtype or g.layout != torch.strided:
-                raise ValueError("AdamW: gradients are dense and in the parameters' dtype")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                kept.append(g)
-            if t["versions"] is not None and t["versions"][i] != p._version:
-                self.state[p]["master"].copy_(p)
-            at.append(i)
-            params.append(p)
-            ps.append(p.data_ptr())
-            gs.append(g.data_ptr())
-        if not at:
-            return
-        rows = t["rows"] if len(at) == len(t["rows"]) else t["rows"][at]
-        rows["p"], rows["g"] = ps, gs
+        params, at = group["params"], None
+        grads = list(map(_GRAD, params))
+        if not all(map(operator.is_not, grads, itertools.repeat(None))):
+            at = [i for i, g in enumerate(grads) if g is not None]
+            params, grads = [params[i] for i in at], [grads[i] for i in at]
+            if not params:
+                return
+        # (checked anew each step, in maps: a network has a hundred tensors, and the step takes 20 us on the GPU)
+        if set(map(_DTYPE, params)) != {dtype} or set(map(_DEVICE, params)) != {device} or not all(map(_DENSE, params)):
+            raise RuntimeError("AdamW: a parameter was moved, cast or restrided since the optimiser was made")
+        if set(map(_DTYPE, grads)) != {dtype} or set(map(_LAYOUT, grads)) != {torch.strided}:
+            raise ValueError("AdamW: gradients are dense and in the parameters' dtype")
+        if not all(map(_DENSE, grads)):
+            grads = [g.contiguous() for g in grads]
+        versions = t["versions"]
+        if versions is not None:
+            for i, p in zip(at or range(len(params)), params):
+                if versions[i] != p._version:
+                    self.state[p]["master"].copy_(p)
+        n = len(params)
+        rows = t["rows"] if at is None else t["rows"][at]
+        rows["p"] = np.fromiter(map(_PTR, params), np.uint64, n)
+        rows["g"] = np.fromiter(map(_PTR, grads), np.uint64, n)
         b1, b2 = group["betas"]
-        _check(_launch(_native.lib().dk_net_adamw_async, device.index, rows.ctypes.data, len(at), _TYPES[dtype], self.state_bits,
+        _check(_launch(_native.lib().dk_net_adamw_async, device.index, rows.ctypes.data, n, _TYPES[dtype], self.state_bits,
                        b["exp_avg"].data_ptr(), b["exp_avg_sq"].data_ptr(), _ptr(b.get("exp_avg_scale")),
                        _ptr(b.get("exp_avg_sq_scale")), _ptr(b.get("master")), b["step"].data_ptr(), t["factors"].data_ptr(),
                        lr, _ptr(d_lr), b1, b2, group["eps"], group["weight_decay"]), "AdamW")
         # the networks' split weights are cached by the parameters' versions
         torch.autograd.graph.increment_version(params)
-        if t["versions"] is not None:
-            for i, p in zip(at, params):
-                t["versions"][i] = p._version
+        if versions is not None:
+            for i, p in zip(at or range(n), params):
+                versions[i] = p._version
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
