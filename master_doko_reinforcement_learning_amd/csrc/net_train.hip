@@ -86,9 +86,8 @@ uint32_t norm_bwd_grid(uint64_t rows, uint32_t d, int type) {
     return n;
 }
 
-// Calls f with the lanes of a row and the elements of each, as types, for vocabularies up to LOGP_SMALL:
-// 16 lanes up to 64 entries (the networks' 33 and 39 classes), a wave up to 1024.
-constexpr uint32_t LOGP_SMALL = 1024;
+// Calls f with the lanes of a row and the elements of each, as types, for small vocabularies: 16 lanes up to
+// 64 entries (the networks' 33 and 39 classes), a wave up to 512.
 template <int G_, int E_>
 struct LogpShape { static constexpr int G = G_, E = E_; };
 template <class F>
@@ -99,19 +98,26 @@ void with_small_vocab(uint32_t vocab, F f) {
     else if (vocab <= 64) f(LogpShape<16, 4>{});
     else if (vocab <= 128) f(LogpShape<64, 2>{});
     else if (vocab <= 256) f(LogpShape<64, 4>{});
-    else if (vocab <= 512) f(LogpShape<64, 8>{});
-    else f(LogpShape<64, 16>{});
+    else f(LogpShape<64, 8>{});
 }
-// Workgroups that share a row: rows alone where they fill the GPU, otherwise parts of at least 2 vectors a thread.
-constexpr uint32_t LOGP_FILL = 1024, LOGP_GRID = 1u << 20;
-struct LogpSplit { uint32_t splits, elems; };
-LogpSplit logp_split(uint64_t rows, uint32_t vocab, int type) {
+// How rows are read: up to LOGP_SMALL entries in the registers of 16 or 64 lanes, unless many alternatives of
+// a vocabulary worth their selection are wanted (20000 x 400 f32: 23 us against 24 for 5 of them, 56 against 25
+// for 20); by a wave each up to 1024 entries (20000 x 1000 bf16: 20 us, 63 with a workgroup each), and up to 8192
+// where the rows fill the GPU (4096 x 3000 bf16: 9 us against 14; 2048 x 20000: 32 against 24); else by a
+// workgroup each, or, where the rows are too few, in parts of at least 2 vectors a thread, a workgroup each.
+constexpr uint32_t LOGP_SMALL = 512, LOGP_FILL = 1024, LOGP_GRID = 1u << 20;
+bool logp_small(uint32_t vocab, uint32_t top) { return vocab <= LOGP_SMALL && (vocab <= 128 || top <= 8); }
+struct LogpPlan { bool small, wave; uint32_t splits, elems; };
+LogpPlan logp_plan(uint64_t rows, uint32_t vocab, int type, uint32_t top) {
+    if (logp_small(vocab, top)) return {true, false, 1u, vocab};
     const uint32_t unit = 256u * (type == DK_F32 ? 4u : 8u);   // a vector a thread
     const uint32_t units = (vocab + unit - 1) / unit;
-    const uint64_t want = rows >= LOGP_FILL ? 1 : LOGP_FILL / (rows ? rows : 1);
-    const uint32_t each = want >= units ? 2u : (uint32_t)((units + want - 1) / want);
-    const uint32_t splits = (units + (each < 2 ? 2 : each) - 1) / (each < 2 ? 2 : each);
-    return {splits, (each < 2 ? 2 : each) * unit};
+    const bool wave = vocab <= 1024 || (rows >= 2048 && vocab <= 8192);
+    if (wave || rows >= LOGP_FILL) return {false, wave, 1u, units * unit};
+    const uint64_t want = LOGP_FILL / (rows ? rows : 1);
+    uint32_t each = (uint32_t)((units + want - 1) / want);
+    each = each < 2 ? 2 : each;
+    return {false, false, (units + each - 1) / each, each * unit};
 }
 uint32_t logp_grid(uint64_t jobs) { return (uint32_t)(jobs < LOGP_GRID ? jobs : LOGP_GRID); }
 
@@ -188,15 +194,15 @@ int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t ro
     if (!logits || (n && (!tokens || !logprobs)) || (top && (!top_logprobs || !top_tokens))) return DK_E_INVALID;
     const uint64_t need = dk_net_token_logprobs_workspace(rows, vocab, type, top);
     if (need && (!workspace || workspace_bytes < need)) return DK_E_INVALID;
-    const LogpSplit split = logp_split(rows, vocab, type);
+    const LogpPlan plan = logp_plan(rows, vocab, type, top);
     float* part = (float*)workspace;
     const LogpArgs a{logits, stride, rows, vocab, n, top, mask, mask_stride, 1.0f / temperature, tokens, logprobs, entropy,
-                     stats, top_logprobs, top_tokens, split.splits, split.elems, part,
-                     (uint64_t*)(part + 4 * rows * split.splits)};
+                     stats, top_logprobs, top_tokens, plan.splits, plan.elems, part,
+                     (uint64_t*)(part + 4 * rows * plan.splits)};
     hipStream_t st = (hipStream_t)stream;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (vocab <= LOGP_SMALL) {
+        if (plan.small) {
             with_small_vocab(vocab, [&](auto s) {
                 using S = decltype(s);
                 hipLaunchKernelGGL((token_logprobs_small_kernel<T, S::G, S::E>), dim3(logp_grid((rows * S::G + 255) / 256)),
@@ -204,8 +210,12 @@ int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t ro
             });
             return;
         }
-        hipLaunchKernelGGL(token_logprobs_kernel<T>, dim3(logp_grid(rows * split.splits)), dim3(256), 0, st, a);
-        if (split.splits > 1) hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3((uint32_t)rows), dim3(256), 0, st, a);
+        const dim3 grid(logp_grid(plan.wave ? (rows + 3) / 4 : rows * plan.splits)), block(256);
+        if (plan.wave && top) hipLaunchKernelGGL((token_logprobs_kernel<T, WAVE, true>), grid, block, 0, st, a);
+        else if (plan.wave) hipLaunchKernelGGL((token_logprobs_kernel<T, WAVE, false>), grid, block, 0, st, a);
+        else if (top) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((token_logprobs_kernel<T, 256, false>), grid, block, 0, st, a);
+        if (plan.splits > 1) hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3((uint32_t)rows), dim3(256), 0, st, a);
     });
     DK_HIP(hipGetLastError());
     return DK_OK;
@@ -213,8 +223,8 @@ int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t ro
 
 // (a row's parts: maximum, S and U of each, then their top entries; none where a workgroup takes a row)
 uint64_t dk_net_token_logprobs_workspace(uint64_t rows, uint32_t vocab, int type, uint32_t top) {
-    if (!type_ok(type) || rows == 0 || vocab <= LOGP_SMALL) return 0;
-    const uint32_t splits = logp_split(rows, vocab, type).splits;
+    if (!type_ok(type) || rows == 0 || vocab == 0) return 0;
+    const uint32_t splits = logp_plan(rows, vocab, type, top).splits;
     return splits > 1 ? rows * splits * (4 * sizeof(float) + top * sizeof(uint64_t)) : 0;
 }
 
@@ -233,7 +243,7 @@ int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_
     hipStream_t st = (hipStream_t)stream;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (vocab <= LOGP_SMALL)
+        if (logp_small(vocab, 0))
             with_small_vocab(vocab, [&](auto s) {
                 using S = decltype(s);
                 hipLaunchKernelGGL((token_logprobs_small_bwd_kernel<T, S::G, S::E>), dim3(logp_grid((rows * S::G + 255) / 256)),

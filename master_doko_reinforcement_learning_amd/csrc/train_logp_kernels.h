@@ -80,30 +80,34 @@ __device__ __forceinline__ RowSoft finish_row(Soft a, float inv_t) {
 // log probability of an allowed logit: of differences, so that a large common offset costs nothing
 __device__ __forceinline__ float logprob_of(float v, const RowSoft& r, float inv_t) { return (v - r.m) * inv_t - r.log_s; }
 
+// a row's token i with its logit: loaded before the sums are, so that the two dependent reads run beside them
+struct Token { float v; bool pad, over; };
 template <class T>
-__device__ __forceinline__ void finish_tokens(const LogpArgs& a, uint64_t row, const RowSoft& r, uint32_t first, uint32_t step) {
-    if (first == 0) {
-        if (a.stats) *(float2*)(a.stats + 2 * row) = make_float2(r.m, r.log_s);
-        if (a.entropy) a.entropy[row] = r.ent;
-    }
-    const T* x = (const T*)a.logits + row * a.stride;
-    for (uint32_t i = first; i < a.n; i += step) {
+__device__ __forceinline__ Token load_token(const LogpArgs& a, uint64_t row, uint32_t i) {
+    Token k{NEG_INF, false, false};
+    if (i < a.n) {
         const int64_t t = a.tokens[row * a.n + i];
-        float v = 0.0f;
-        if (t >= (int64_t)a.vocab) v = __builtin_nanf("");
-        else if (t >= 0) {
-            v = a.mask && !a.mask[row * a.mask_stride + t] ? NEG_INF : to_f32(x[t]);
-            v = v != NEG_INF ? logprob_of(v, r, a.inv_t) : r.log_s != r.log_s ? r.log_s : NEG_INF;
-        }
-        a.logprobs[row * a.n + i] = v;
+        k.pad = t < 0;
+        k.over = t >= (int64_t)a.vocab;
+        if (!k.pad && !k.over && (!a.mask || a.mask[row * a.mask_stride + t])) k.v = to_f32(((const T*)a.logits)[row * a.stride + t]);
     }
+    return k;
+}
+__device__ __forceinline__ void finish_token(const LogpArgs& a, uint64_t row, uint32_t i, const Token& k, const RowSoft& r) {
+    if (i >= a.n) return;
+    const float none = r.log_s != r.log_s ? r.log_s : NEG_INF;
+    a.logprobs[row * a.n + i] = k.pad ? 0.0f : k.over ? __builtin_nanf("") : k.v == NEG_INF ? none : logprob_of(k.v, r, a.inv_t);
+}
+__device__ __forceinline__ void finish_stats(const LogpArgs& a, uint64_t row, const RowSoft& r) {
+    if (a.stats) *(float2*)(a.stats + 2 * row) = make_float2(r.m, r.log_s);
+    if (a.entropy) a.entropy[row] = r.ent;
 }
 __device__ __forceinline__ void finish_top(const LogpArgs& a, uint64_t row, const RowSoft& r, uint32_t k, uint64_t e) {
     a.top_tokens[row * a.top + k] = e ? (int64_t)(uint32_t)~(uint32_t)e : -1;
     a.top_logprobs[row * a.top + k] = e ? logprob_of(key_value((uint32_t)(e >> 32)), r, a.inv_t) : r.log_s != r.log_s ? r.log_s : NEG_INF;
 }
 
-// Vocabularies up to 1024: G lanes share a row, E elements each in registers, 256 / G rows a workgroup.
+// Vocabularies up to 512: G lanes share a row, E elements each in registers, 256 / G rows a workgroup.
 template <class T, int G, int E>
 __global__ __launch_bounds__(256) void token_logprobs_small_kernel(LogpArgs a) {
     const uint32_t lane = threadIdx.x % G;
@@ -125,6 +129,7 @@ __global__ __launch_bounds__(256) void token_logprobs_small_kernel(LogpArgs a) {
                 if (at < a.vocab && !mask[at]) v[i] = NEG_INF;
             }
         }
+        const Token token = load_token<T>(a, row, lane);
         float m = LOWEST;
 #pragma unroll
         for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
@@ -137,7 +142,8 @@ __global__ __launch_bounds__(256) void token_logprobs_small_kernel(LogpArgs a) {
             u += fmaxf(z, LOWEST) * e;
         }
         const RowSoft r = finish_row({m, lanes_reduce<G, Add>(s), lanes_reduce<G, Add>(u)}, a.inv_t);
-        finish_tokens<T>(a, row, r, lane, G);
+        if (lane == 0) finish_stats(a, row, r);
+        for (uint32_t i = lane; i < a.n; i += G) finish_token(a, row, i, i == lane ? token : load_token<T>(a, row, i), r);
         if (a.top == 0) continue;
         uint32_t key[E];
 #pragma unroll
@@ -158,44 +164,61 @@ __global__ __launch_bounds__(256) void token_logprobs_small_kernel(LogpArgs a) {
     }
 }
 
-// The k largest of a workgroup's entries, sorted, in out[0 .. k) (0 behind the last).  `mine` is the largest
+// W threads that share a row: a workgroup of 4 waves, or a wave
+template <int W>
+__device__ __forceinline__ void team_sync() {
+    if constexpr (W > WAVE) __syncthreads();
+    else {   // (a wave's LDS accesses are done in order: the compiler must keep them so)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The k largest of a team's entries, sorted, in lds.top[0 .. k) (0 behind the last).  `mine` is the largest
 // key among a thread's entries; scan(least, push) goes through the entries of the threads whose mine is at
 // least `least` and pushes those whose key is; best(below) is the thread's largest entry under `below`.
 //   Of a wave's threads at least k have mine >= T for the k-th largest T of them, so no entry below any
 // wave's T is among the k largest: the others are few, except where many are equal.
+template <int W>
 struct TopLds {
-    static constexpr uint32_t ROOM = 1024;
-    uint64_t e[ROOM];
-    uint32_t least[4], count;
-    uint64_t best[4];
+    static constexpr uint32_t ROOM = W > WAVE ? 1024 : 256;
+    uint64_t e[ROOM + 8], top[TOP_MAX], best[4];
+    uint32_t least[4], count, n_winners, winners[W];
 };
-template <int BITS, class Scan, class Best>
-__device__ __forceinline__ void block_top(uint32_t k, uint32_t mine, TopLds& lds, uint64_t* out, Scan scan, Best best) {
+template <int W, int BITS, class Scan, class Best>
+__device__ __forceinline__ void team_top(uint32_t k, uint32_t mine, TopLds<W>& lds, Scan scan, Best best) {
+    const uint32_t tid = threadIdx.x % W;
     uint32_t least = 0;
     for (int b = 31; b >= 32 - BITS; --b) {
         const uint32_t next = least | 1u << b;
         if ((uint32_t)__popcll(__ballot(mine >= next)) >= k) least = next;
     }
-    __syncthreads();
-    if (threadIdx.x % WAVE == 0) lds.least[threadIdx.x / WAVE] = least;
-    if (threadIdx.x == 0) lds.count = 0;
-    __syncthreads();
-    least = 1;
-    for (int i = 0; i < 4; ++i) least = lds.least[i] > least ? lds.least[i] : least;
+    if constexpr (W > WAVE) {
+        if (tid % WAVE == 0) lds.least[tid / WAVE] = least;
+    }
+    if (tid == 0) lds.count = 0;
+    team_sync<W>();
+    if constexpr (W > WAVE)
+        for (int i = 0; i < W / WAVE; ++i) least = lds.least[i] > least ? lds.least[i] : least;
+    if (least == 0) least = 1;
     scan(least, [&](uint32_t key, uint32_t index) {
         const uint32_t at = atomicAdd(&lds.count, 1u);   // (any order: the ranks below depend on the set alone)
-        if (at < TopLds::ROOM) lds.e[at] = entry(key, index);
+        if (at < TopLds<W>::ROOM) lds.e[at] = entry(key, index);
     });
-    __syncthreads();
+    team_sync<W>();
     const uint32_t count = lds.count;
-    if (count <= TopLds::ROOM) {
-        for (uint32_t i = threadIdx.x; i < count; i += 256) {
+    if (count <= TopLds<W>::ROOM) {
+        if (tid < 8) lds.e[count + tid] = 0;   // (whole groups of 8 below)
+        team_sync<W>();
+        for (uint32_t i = tid; i < count; i += W) {
             const uint64_t e = lds.e[i];
             uint32_t rank = 0;
-            for (uint32_t j = 0; j < count; ++j) rank += lds.e[j] > e;
-            if (rank < k) out[rank] = e;
+            for (uint32_t j = 0; j < count; j += 8)
+#pragma unroll
+                for (int l = 0; l < 8; ++l) rank += lds.e[j + l] > e;
+            if (rank < k) lds.top[rank] = e;
         }
-        for (uint32_t i = count + threadIdx.x; i < k; i += 256) out[i] = 0;
+        for (uint32_t i = count + tid; i < k; i += W) lds.top[i] = 0;
     } else {   // more equal ones than there is room: one after the other
         uint64_t last = ~0ull;
         for (uint32_t r = 0; r < k; ++r) {
@@ -204,26 +227,30 @@ __device__ __forceinline__ void block_top(uint32_t k, uint32_t mine, TopLds& lds
                 const uint64_t w = __shfl_xor((unsigned long long)e, o);
                 e = w > e ? w : e;
             }
-            __syncthreads();
-            if (threadIdx.x % WAVE == 0) lds.best[threadIdx.x / WAVE] = e;
-            __syncthreads();
-            for (int i = 0; i < 4; ++i) e = lds.best[i] > e ? lds.best[i] : e;
-            if (threadIdx.x == 0) out[r] = e;
+            if constexpr (W > WAVE) {
+                team_sync<W>();
+                if (tid % WAVE == 0) lds.best[tid / WAVE] = e;
+                team_sync<W>();
+                for (int i = 0; i < W / WAVE; ++i) e = lds.best[i] > e ? lds.best[i] : e;
+            }
+            if (tid == 0) lds.top[r] = e;
             last = e;
         }
     }
-    __syncthreads();
+    team_sync<W>();
 }
 
-// S and U of a workgroup's threads together; `lds` has 4 entries
-__device__ __forceinline__ Soft block_soft(Soft a, float c, Soft* lds) {
-    a = lanes_soft<64>(a, c);
+// S and U of a team's threads together; `lds` has 4 entries
+template <int W>
+__device__ __forceinline__ Soft team_soft(Soft a, float c, Soft* lds) {
+    a = lanes_soft<WAVE>(a, c);
+    if constexpr (W == WAVE) return a;
     if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = a;
     __syncthreads();
     float m = lds[0].m;
-    for (int i = 1; i < 4; ++i) m = fmaxf(m, lds[i].m);
+    for (int i = 1; i < W / WAVE; ++i) m = fmaxf(m, lds[i].m);
     Soft r{m, 0.0f, 0.0f};
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W / WAVE; ++i) {
         const Soft w = rebased(lds[i], m, c);
         r.s += w.s;
         r.u += w.u;
@@ -235,10 +262,10 @@ __device__ __forceinline__ Soft block_soft(Soft a, float c, Soft* lds) {
 template <class T>
 using MaskVec __attribute__((aligned(1))) = uint8_t __attribute__((ext_vector_type(VEC<T>)));
 
-// VEC logits from column at on as f32, -inf for what is masked or behind the row's end
+// VEC logits from column at on as f32, -inf for what is masked or not below hi
 template <class T, bool WHOLE>
-__device__ __forceinline__ void load_logits(const T* x, const uint8_t* mask, uint32_t at, uint32_t vocab, float* v) {
-    if (WHOLE || at + VEC<T> <= vocab) {
+__device__ __forceinline__ void load_logits(const T* x, const uint8_t* mask, uint32_t at, uint32_t hi, float* v) {
+    if (WHOLE || at + VEC<T> <= hi) {
         const Vec<T> raw = *(const Vec<T>*)(x + at);
 #pragma unroll
         for (int j = 0; j < VEC<T>; ++j) v[j] = to_f32((T)raw[j]);
@@ -249,29 +276,34 @@ __device__ __forceinline__ void load_logits(const T* x, const uint8_t* mask, uin
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < VEC<T>; ++j) v[j] = at + j < vocab && (!mask || mask[at + j]) ? to_f32(x[at + j]) : NEG_INF;
+        for (int j = 0; j < VEC<T>; ++j)
+            v[j] = at + j < hi && (!mask || mask[at + j]) ? to_f32(x[at + j]) : NEG_INF;
     }
 }
 
-// Larger vocabularies: a workgroup goes once through a row, or through one of its `splits` parts where the
-// rows are too few to fill the GPU, each thread with a running maximum (rebased every 4 vectors).  The top
-// entries lie with the threads of the largest maxima: their elements alone are read again.
-template <class T>
+// Larger vocabularies: W threads go once through a row, or a workgroup through one of its `splits` parts
+// where the rows are too few to fill the GPU, each thread with a running maximum (rebased every 16 elements:
+// 4096 x 65536 bf16 takes 103 us so, 5.2 TB/s, 107 us with 32, whose registers cost waves).  The top entries
+// lie with the threads of the largest maxima: their elements alone are read again.  Without them (TOP false)
+// the kernel has half the registers: 103 us against 118.
+template <class T, int W, bool TOP>
 __global__ __launch_bounds__(256) void token_logprobs_kernel(LogpArgs a) {
-    constexpr int V = VEC<T>, B = 4;
+    constexpr int V = VEC<T>, B = 16 / V, TEAMS = 256 / W;
     __shared__ Soft soft_lds[4];
-    __shared__ TopLds top_lds;
-    __shared__ uint64_t top[TOP_MAX];
-    __shared__ uint32_t winners[256], n_winners;
+    __shared__ TopLds<W> top_lds[TEAMS];
+    TopLds<W>& lds = top_lds[threadIdx.x / W];
+    const uint32_t tid = threadIdx.x % W;
     const float c = a.inv_t * LOG2E;
     const uint64_t jobs = a.rows * a.splits;
-    for (uint64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const uint64_t row = job / a.splits;
-        const uint32_t part = (uint32_t)(job % a.splits);
+    for (uint64_t job = (uint64_t)blockIdx.x * TEAMS + threadIdx.x / W; job < jobs; job += (uint64_t)gridDim.x * TEAMS) {
+        const uint64_t row = W == WAVE ? job : job / a.splits;
+        const uint32_t part = W == WAVE ? 0 : (uint32_t)(job % a.splits);
         const T* x = (const T*)a.logits + row * a.stride;
         const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
         const uint32_t lo = part * a.part_elems, hi = a.vocab - lo > a.part_elems ? lo + a.part_elems : a.vocab;
-        const uint32_t rounds = (hi - lo + 256 * V - 1) / (256 * V);   // vectors of a thread
+        const uint32_t rounds = (hi - lo + W * V - 1) / (W * V);   // (vectors of a thread)
+        Token token{};
+        if (a.splits == 1) token = load_token<T>(a, row, tid);   // (at most 64 tokens)
         Soft mine{LOWEST, 0.0f, 0.0f};
         auto take = [&](const float* v, int n) {
             float m = mine.m;
@@ -285,31 +317,33 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogpArgs a) {
                 mine.u += fmaxf(z, LOWEST) * e;
             }
         };
-        uint32_t q = 0;
-        for (; (q + B) * 256 * V <= hi - lo; q += B) {
-            float v[B * V];
+        uint32_t first = lo;
+        float v[B * V];
+        for (; hi - first >= B * W * V; first += B * W * V) {
 #pragma unroll
-            for (int i = 0; i < B; ++i) load_logits<T, true>(x, mask, lo + ((q + i) * 256 + threadIdx.x) * V, hi, v + i * V);
+            for (int i = 0; i < B; ++i) load_logits<T, true>(x, mask, first + (i * W + tid) * V, hi, v + i * V);
             take(v, B * V);
         }
-        for (; q < rounds; ++q) {
-            float v[V];
-            load_logits<T, false>(x, mask, lo + (q * 256 + threadIdx.x) * V, hi, v);
-            take(v, V);
-        }
+        // the rest, less than B vectors a thread: all loads first, then the sums of those that there are
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (first + (i * W + tid) * V < hi) load_logits<T, false>(x, mask, first + (i * W + tid) * V, hi, v + i * V);
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (first + (i * W + tid) * V < hi) take(v + i * V, V);
         const uint32_t key = mine.s == 0.0f ? 0u : order_key(mine.m);
-        const Soft all = block_soft(mine, c, soft_lds);
-        if (a.top)
-            block_top<KEY_BITS<T>>(
-                a.top, key, top_lds, top,
+        const Soft all = team_soft<W>(mine, c, soft_lds);
+        if constexpr (TOP)
+            team_top<W, KEY_BITS<T>>(
+                a.top, key, lds,
                 [&](uint32_t least, auto push) {
-                    if (threadIdx.x == 0) n_winners = 0;
-                    __syncthreads();
-                    if (key >= least) winners[atomicAdd(&n_winners, 1u)] = threadIdx.x;
-                    __syncthreads();
-                    const uint32_t vectors = n_winners * rounds;
-                    for (uint32_t i = threadIdx.x; i < vectors; i += 256) {
-                        const uint32_t at = lo + (i % rounds * 256 + winners[i / rounds]) * V;
+                    if (tid == 0) lds.n_winners = 0;
+                    team_sync<W>();
+                    if (key >= least) lds.winners[atomicAdd(&lds.n_winners, 1u)] = tid;
+                    team_sync<W>();
+                    const uint32_t vectors = lds.n_winners * rounds;
+                    for (uint32_t i = tid; i < vectors; i += W) {
+                        const uint32_t at = lo + (i % rounds * W + lds.winners[i / rounds]) * V;
                         float v[V];
                         load_logits<T, false>(x, mask, at, hi, v);
 #pragma unroll
@@ -322,7 +356,7 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogpArgs a) {
                 [&](uint64_t below) {
                     uint64_t best = 0;
                     for (uint32_t i = 0; i < rounds; ++i) {
-                        const uint32_t at = lo + (i * 256 + threadIdx.x) * V;
+                        const uint32_t at = lo + (i * W + tid) * V;
                         float v[V];
                         load_logits<T, false>(x, mask, at, hi, v);
 #pragma unroll
@@ -335,13 +369,14 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogpArgs a) {
                 });
         if (a.splits == 1) {
             const RowSoft r = finish_row(all, a.inv_t);
-            finish_tokens<T>(a, row, r, threadIdx.x, 256);
-            if (threadIdx.x < a.top) finish_top(a, row, r, threadIdx.x, top[threadIdx.x]);
+            if (tid == 0) finish_stats(a, row, r);
+            finish_token(a, row, tid, token, r);
+            if (TOP && tid < a.top) finish_top(a, row, r, tid, lds.top[tid]);
         } else {
-            if (threadIdx.x == 0) *(float4*)(a.part + 4 * job) = make_float4(all.m, all.s, all.u, 0.0f);
-            if (threadIdx.x < a.top) a.part_top[job * a.top + threadIdx.x] = top[threadIdx.x];
+            if (tid == 0) *(float4*)(a.part + 4 * job) = make_float4(all.m, all.s, all.u, 0.0f);
+            if (TOP && tid < a.top) a.part_top[job * a.top + tid] = lds.top[tid];
         }
-        __syncthreads();
+        team_sync<W>();
     }
 }
 
@@ -349,10 +384,17 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogpArgs a) {
 template <class T>
 __global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogpArgs a) {
     __shared__ Soft soft_lds[4];
-    __shared__ TopLds top_lds;
-    __shared__ uint64_t top[TOP_MAX];
+    __shared__ TopLds<256> lds;
     const uint64_t row = blockIdx.x;
     const float c = a.inv_t * LOG2E;
+    const uint64_t* e = a.part_top + row * a.splits * a.top;
+    const uint32_t n = a.splits * a.top;
+    uint32_t key = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        const uint32_t k = (uint32_t)(e[i] >> 32);
+        key = k > key ? k : key;
+    }
+    const Token token = load_token<T>(a, row, threadIdx.x);
     Soft mine{LOWEST, 0.0f, 0.0f};
     for (uint32_t i = threadIdx.x; i < a.splits; i += 256) {
         const float4 p = *(const float4*)(a.part + 4 * (row * a.splits + i));
@@ -362,21 +404,17 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogpArgs a) {
         mine.s += s.s;
         mine.u += s.u;
     }
-    const RowSoft r = finish_row(block_soft(mine, c, soft_lds), a.inv_t);
-    finish_tokens<T>(a, row, r, threadIdx.x, 256);
+    const RowSoft r = finish_row(team_soft<256>(mine, c, soft_lds), a.inv_t);
+    if (threadIdx.x == 0) finish_stats(a, row, r);
+    finish_token(a, row, threadIdx.x, token, r);
     if (a.top == 0) return;
-    const uint64_t* e = a.part_top + row * a.splits * a.top;
-    const uint32_t n = a.splits * a.top;
-    uint32_t key = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
-        const uint32_t k = (uint32_t)(e[i] >> 32);
-        key = k > key ? k : key;
-    }
-    block_top<KEY_BITS<T>>(
-        a.top, key, top_lds, top,
+    team_top<256, KEY_BITS<T>>(
+        a.top, key, lds,
         [&](uint32_t least, auto push) {
-            for (uint32_t i = threadIdx.x; i < n; i += 256)
-                if ((uint32_t)(e[i] >> 32) >= least) push((uint32_t)(e[i] >> 32), ~(uint32_t)e[i]);
+            for (uint32_t i = threadIdx.x; i < n; i += 256) {
+                const uint64_t w = e[i];
+                if ((uint32_t)(w >> 32) >= least) push((uint32_t)(w >> 32), ~(uint32_t)w);
+            }
         },
         [&](uint64_t below) {
             uint64_t best = 0;
@@ -384,7 +422,7 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogpArgs a) {
                 if (e[i] < below && e[i] > best) best = e[i];
             return best;
         });
-    if (threadIdx.x < a.top) finish_top(a, row, r, threadIdx.x, top[threadIdx.x]);
+    if (threadIdx.x < a.top) finish_top(a, row, r, threadIdx.x, lds.top[threadIdx.x]);
 }
 
 struct LogpBwdArgs {
@@ -478,7 +516,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(LogpBwdArgs a) 
     const uint32_t n = a.dlogp ? a.n : 0;
     const uint64_t jobs = a.rows * a.parts;
     for (uint64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const uint64_t row = job / a.parts;
+        const uint64_t row = a.rows - 1 - job / a.parts;   // from the end: what the forward pass read last is still in the cache
         const uint32_t lo = (uint32_t)(job % a.parts) * (256 * V * B);
         const T* x = (const T*)a.logits + row * a.stride;
         const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
