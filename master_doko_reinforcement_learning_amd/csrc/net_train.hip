@@ -102,17 +102,19 @@ void with_small_vocab(uint32_t vocab, F f) {
 }
 // How rows are read: up to LOGP_SMALL entries in the registers of 16 or 64 lanes, unless many alternatives of
 // a vocabulary worth their selection are wanted (20000 x 400 f32: 23 us against 24 for 5 of them, 56 against 25
-// for 20); by a wave each up to 1024 entries (20000 x 1000 bf16: 20 us, 63 with a workgroup each), and up to 8192
+// for 20); by a wave each up to 1024 entries (20000 x 1000 bf16: 20 us, 63 with a workgroup each), and up to LOGP_WAVE
 // where the rows fill the GPU (4096 x 3000 bf16: 9 us against 14; 2048 x 20000: 32 against 24); else by a
 // workgroup each, or, where the rows are too few, in parts of at least 2 vectors a thread, a workgroup each.
-constexpr uint32_t LOGP_SMALL = 512, LOGP_FILL = 1024, LOGP_GRID = 1u << 20;
+// The backward pass takes parts of 4 vectors a thread, a wave's up to LOGP_WAVE entries (20000 x 1000 bf16: 27 us
+// against 49; 20000 x 8000 f32: 248 against 267), beyond that a workgroup's (20000 x 20000 bf16: 333 against 362).
+constexpr uint32_t LOGP_SMALL = 512, LOGP_WAVE = 8192, LOGP_FILL = 1024, LOGP_GRID = 1u << 20;
 bool logp_small(uint32_t vocab, uint32_t top) { return vocab <= LOGP_SMALL && (vocab <= 128 || top <= 8); }
 struct LogpPlan { bool small, wave; uint32_t splits, elems; };
 LogpPlan logp_plan(uint64_t rows, uint32_t vocab, int type, uint32_t top) {
     if (logp_small(vocab, top)) return {true, false, 1u, vocab};
     const uint32_t unit = 256u * (type == DK_F32 ? 4u : 8u);   // a vector a thread
     const uint32_t units = (vocab + unit - 1) / unit;
-    const bool wave = vocab <= 1024 || (rows >= 2048 && vocab <= 8192);
+    const bool wave = vocab <= 1024 || (rows >= 2048 && vocab <= LOGP_WAVE);
     if (wave || rows >= LOGP_FILL) return {false, wave, 1u, units * unit};
     const uint64_t want = LOGP_FILL / (rows ? rows : 1);
     uint32_t each = (uint32_t)((units + want - 1) / want);
@@ -237,7 +239,8 @@ int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
     if (!logits || (n && (!tokens || !logprobs)) || !stats || !entropy || !dlogits) return DK_E_INVALID;
-    const uint32_t unit = 256u * 4u * (type == DK_F32 ? 4u : 8u), parts = (vocab + unit - 1) / unit;
+    const bool wave = vocab <= LOGP_WAVE;
+    const uint32_t unit = (wave ? 64u : 256u) * 4u * (type == DK_F32 ? 4u : 8u), parts = (vocab + unit - 1) / unit;
     const LogpBwdArgs a{logits, stride, rows, vocab, n, mask, mask_stride, 1.0f / temperature, tokens, logprobs, stats, entropy,
                         dlogprobs, dentropy, dlogits, parts};
     hipStream_t st = (hipStream_t)stream;
@@ -249,8 +252,10 @@ int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_
                 hipLaunchKernelGGL((token_logprobs_small_bwd_kernel<T, S::G, S::E>), dim3(logp_grid((rows * S::G + 255) / 256)),
                                    dim3(256), 0, st, a);
             });
+        else if (wave)
+            hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, WAVE>), dim3(logp_grid((rows * parts + 3) / 4)), dim3(256), 0, st, a);
         else
-            hipLaunchKernelGGL(token_logprobs_bwd_kernel<T>, dim3(logp_grid(rows * parts)), dim3(256), 0, st, a);
+            hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 256>), dim3(logp_grid(rows * parts)), dim3(256), 0, st, a);
     });
     DK_HIP(hipGetLastError());
     return DK_OK;

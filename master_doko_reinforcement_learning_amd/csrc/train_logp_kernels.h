@@ -506,55 +506,58 @@ __global__ __launch_bounds__(256) void token_logprobs_small_bwd_kernel(LogpBwdAr
     }
 }
 
-// larger vocabularies: a workgroup takes 4 vectors a thread of a row.  The tokens' columns are written
-// again at the end, each by the first of its equal tokens with all their gradients in order.
-template <class T>
+// Larger vocabularies: W threads take 4 vectors each of a row.  The tokens' columns are written again at the
+// end, each by the first of its equal tokens with all their gradients in order.
+template <class T, int W>
 __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(LogpBwdArgs a) {
-    constexpr int V = VEC<T>, B = 4;
-    __shared__ int32_t tok[TOKENS_MAX];
-    __shared__ float grad[TOKENS_MAX];
-    const uint32_t n = a.dlogp ? a.n : 0;
+    constexpr int V = VEC<T>, B = 4, TEAMS = 256 / W;
+    __shared__ int32_t team_tok[TEAMS][TOKENS_MAX];
+    __shared__ float team_grad[TEAMS][TOKENS_MAX];
+    const uint32_t tid = threadIdx.x % W, n = a.dlogp ? a.n : 0;
+    int32_t* tok = team_tok[threadIdx.x / W];
+    float* grad = team_grad[threadIdx.x / W];
     const uint64_t jobs = a.rows * a.parts;
-    for (uint64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const uint64_t row = a.rows - 1 - job / a.parts;   // from the end: what the forward pass read last is still in the cache
-        const uint32_t lo = (uint32_t)(job % a.parts) * (256 * V * B);
+    for (uint64_t job = (uint64_t)blockIdx.x * TEAMS + threadIdx.x / W; job < jobs; job += (uint64_t)gridDim.x * TEAMS) {
+        const uint64_t row = a.rows - 1 - job / a.parts;   // from the end: what the forward pass read last may still be in the cache
+        const uint32_t lo = (uint32_t)(job % a.parts) * (W * V * B);
         const T* x = (const T*)a.logits + row * a.stride;
         const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
         float v[B][V];
-        const bool whole = lo + 256 * V * B <= a.vocab;
+        const bool whole = lo + W * V * B <= a.vocab;
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            const uint32_t at = lo + (i * 256 + threadIdx.x) * V;
+            const uint32_t at = lo + (i * W + tid) * V;
             if (whole) load_logits<T, true>(x, mask, at, a.vocab, v[i]);
-            else load_logits<T, false>(x, mask, at, a.vocab, v[i]);
+            else if (at < a.vocab) load_logits<T, false>(x, mask, at, a.vocab, v[i]);
         }
-        if (threadIdx.x < n) grad[threadIdx.x] = token_gradient(a, row, threadIdx.x, tok[threadIdx.x]);
-        __syncthreads();
+        if (tid < n) grad[tid] = token_gradient(a, row, tid, tok[tid]);
+        team_sync<W>();
         float total = 0.0f;
         for (uint32_t k = 0; k < n; ++k) total += grad[k];
         const RowGrad r = row_gradient(a, row, total);
         T* dx = (T*)a.dx + row * a.vocab;
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            const uint32_t at = lo + (i * 256 + threadIdx.x) * V;
+            const uint32_t at = lo + (i * W + tid) * V;
+            if (!whole && at >= a.vocab) continue;
             Vec<T> o;
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = from_f32<T>(r.of(v[i][j]) * a.inv_t);
             if (whole) *(Vec<T>*)(dx + at) = o;
-            else if (at < a.vocab) store_vec(dx, at, a.vocab, o);
+            else store_vec(dx, at, a.vocab, o);
         }
-        __syncthreads();   // (the columns' first values are written before their last)
-        if (threadIdx.x < n) {
-            const int32_t t = tok[threadIdx.x];
-            bool first = t >= 0 && (uint32_t)t >= lo && (uint32_t)t - lo < 256 * V * B;
-            for (uint32_t k = 0; k < threadIdx.x; ++k) first = first && tok[k] != t;
+        team_sync<W>();   // (the columns' first values are written before their last)
+        if (tid < n) {
+            const int32_t t = tok[tid];
+            bool first = t >= 0 && (uint32_t)t >= lo && (uint32_t)t - lo < W * V * B;
+            for (uint32_t k = 0; k < tid; ++k) first = first && tok[k] != t;
             if (first) {
                 float d = r.of(to_f32(x[t]));
-                for (uint32_t k = threadIdx.x; k < n; ++k) d += tok[k] == t ? grad[k] : 0.0f;
+                for (uint32_t k = tid; k < n; ++k) d += tok[k] == t ? grad[k] : 0.0f;
                 dx[t] = from_f32<T>(d * a.inv_t);
             }
         }
-        __syncthreads();
+        team_sync<W>();
     }
 }
 
