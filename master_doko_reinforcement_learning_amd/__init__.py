@@ -19,14 +19,14 @@ __all__ = ["Engine", "McEnv", "CachedMCTS", "SmallRng", "card_matching_full", "s
            "fdo_from_fields", "fdo_to_fields", "do_from_fields", "do_to_fields", "ttt_state",
            "tic_tac_toe_player", "tic_tac_toe_games"]
 
-# the networks' training operators (net_ops.py), on first use: the search alone does not need torch
-_NET_OPS = ("layer_norm", "token_logprobs", "TokenLogprobs", "AdamW")
+# the networks' training operators, on first use: the search alone does not need torch
+_NET_OPS = {"layer_norm": "net_ops", "token_logprobs": "net_ops", "TokenLogprobs": "net_ops", "AdamW": "net_ops", "NetTrainer": "net_trainer"}
 
 
 def __getattr__(name):
     if name in _NET_OPS:
-        from . import net_ops
-        return getattr(net_ops, name)
+        import importlib
+        return getattr(importlib.import_module("." + _NET_OPS[name], __name__), name)
     raise AttributeError("module %r has no attribute %r" % (__name__, name))
 
 

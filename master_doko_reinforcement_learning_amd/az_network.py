@@ -494,6 +494,27 @@ class FusedTrunkF32(FusedTrunk):
         return self.add_ln(x, _f32c(F.linear(a, blk.proj.weight)), ln, blk.proj.bias)
 
 
+def embed_tokens(emb, tokens):
+    """x = the six token embeddings' sum [B, 62, d] (differentiable; the trunks' embedding, left to right)."""
+    t = tokens.long()
+    return sum(emb[i](t[:, SEQ * i:SEQ * (i + 1)]) for i in range(5)) + emb[5](t[:, 310:311])
+
+
+def norm_train(x, ln, delta=None):
+    """ln(x), or (x + delta, ln(x + delta)), on the GPU with its gradient (net_ops.layer_norm)."""
+    from .net_ops import layer_norm
+    return layer_norm(x, ln.weight, ln.bias, ln.eps, delta=delta)
+
+
+def trunk_train(x, h, blocks, final_ln):
+    """The blocks on the residual stream x with h = blocks[0].ln_1(x), differentiable: each residual add runs
+    fused with the LayerNorm after it, forward and backward.  Returns (x, final_ln(x))."""
+    for i, blk in enumerate(blocks):
+        x, h = norm_train(x, blk.ln_2, blk.attn_delta(h))
+        x, h = norm_train(x, blocks[i + 1].ln_1 if i + 1 < len(blocks) else final_ln, blk.mlp_delta(h))
+    return x, h
+
+
 class DokoAzNet(nn.Module):
     def __init__(self, d=160, heads=4, layers=4, policy_layers=1, value_layers=1):
         super().__init__()
@@ -525,6 +546,29 @@ class DokoAzNet(nn.Module):
         for blk in self.v_blocks:
             xv = blk(xv)
         return self.value_head(self.v_ln(xv), fused=False), self.policy_head(self.p_ln(xp), fused=False)
+
+    def forward_train(self, tokens):
+        """The differentiable forward on the GPU (f32): forward_torch with every residual add and LayerNorm of
+        the blocks in one kernel, forward and backward.  tokens [B, 311] -> (value [B, 4], logits [B, 39])."""
+        if not (self.blocks and self.p_blocks and self.v_blocks):
+            raise ValueError("the training forward needs shared, policy and value blocks")
+        x = embed_tokens(self.emb, tokens)
+        x, hp = trunk_train(x, norm_train(x, self.blocks[0].ln_1), self.blocks, self.p_blocks[0].ln_1)
+        _, hv = trunk_train(x, norm_train(x, self.v_blocks[0].ln_1), self.v_blocks, self.v_ln)
+        _, hp = trunk_train(x, hp, self.p_blocks, self.p_ln)
+        return self.value_head(hv, fused=False), self.policy_head(hp, fused=False)
+
+    def loss(self, tokens, value, policy, mask=None, entropy=0.0):
+        """The AlphaZero loss of a batch: the mean squared error of the values [B, 4] plus the mean cross entropy of
+        the policies [B, 39] (the searches' visit shares) under the legal actions `mask` [B, 39], less `entropy` times
+        the policies' mean entropy.  A target on an action that is not allowed does not count."""
+        from .net_ops import token_logprobs
+        v, logits = self.forward_train(tokens)
+        actions = torch.arange(logits.shape[1], device=logits.device).expand(logits.shape)
+        got = token_logprobs(logits, actions, mask=mask)
+        wanted = policy > 0 if mask is None else (policy > 0) & mask
+        ce = -torch.where(wanted, policy * got.logprobs, 0.0).sum(-1).mean()
+        return F.mse_loss(v, value) + ce - entropy * got.entropy.mean()
 
     def forward_fused(self, tokens, trunk=None):
         """bf16 forward on the GPU with HIP kernels (csrc/az_net_kernels.h): the embedding

@@ -18,7 +18,7 @@ load_reference_state_dict maps a reference state_dict onto this module.
 import torch
 from torch import nn
 
-from .az_network import SEQ, Block, ClassHead, FusedTrunk, FusedTrunkF32, f32_fused_ok
+from .az_network import SEQ, Block, ClassHead, FusedTrunk, FusedTrunkF32, embed_tokens, f32_fused_ok, norm_train, trunk_train
 
 VOCAB_IPI = (43, 57, 5, 13, 3, 5)   # object, position, player, subposition, team, player to guess (main.py:91-96)
 IPI_CLASSES = 33
@@ -45,6 +45,28 @@ class DokoImpiNet(nn.Module):
         for blk in self.blocks:
             x = blk(x)
         return self.head(self.ln_f(x), fused=False)
+
+    def forward_train(self, tokens):
+        """The differentiable forward on the GPU (f32): forward_torch with every residual add and LayerNorm of
+        the blocks in one kernel, forward and backward."""
+        x = embed_tokens(self.emb, tokens)
+        _, h = trunk_train(x, norm_train(x, self.blocks[0].ln_1), self.blocks, self.ln_f)
+        return self.head(h, fused=False)
+
+    def loss(self, tokens, guesses, mask=None):
+        """Mean cross entropy of the guesses [B] (ImperfectInformationOutput classes; negative: not counted) under
+        the consistent classes `mask` [B, 33]."""
+        from .net_ops import token_logprobs
+        lp = token_logprobs(self.forward_train(tokens), guesses, mask=mask).logprobs
+        return -lp.sum() / (guesses >= 0).sum().clamp(min=1)
+
+    @torch.no_grad()
+    def logprobs(self, tokens, guesses=None, mask=None, temperature=1.0, top=0):
+        """Log probabilities of given guesses [B] (or [B, n]) as the sampler draws them (softmax(logits / temperature)
+        over the consistent classes `mask`), with the rows' entropy and their `top` likeliest classes
+        (net_ops.TokenLogprobs)."""
+        from .net_ops import token_logprobs
+        return token_logprobs(self(tokens), guesses, mask=mask, temperature=temperature, top=top)
 
     def forward_fused(self, tokens, trunk=None):
         d = self.emb[0].weight.shape[1]
