@@ -15,29 +15,34 @@ LIB_PATH = os.path.join(PKG_DIR, "libdoko_amd.so")
 PROF_LIB_PATH = os.path.join(PKG_DIR, "libdoko_amd_prof.so")
 SRC = os.path.join(PKG_DIR, "csrc", "doko_amd.hip")
 TRAIN_SRC = os.path.join(PKG_DIR, "csrc", "net_train.hip")
-HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared"]
-# the training operators: no packed f32 instructions (the host pass warns that it does not know the feature)
-TRAIN_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# No packed f32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results.
+# hipcc's host pass warns that it does not know the feature: that is harmless.
+ARCH_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# the translation units, with the options of each (the search is bit-exact with its restatement: its products
+# are not fused into sums)
+UNITS = ((SRC, ["-ffp-contract=off"]), (TRAIN_SRC, []))
 
 
 def build(verbose=False, profiling=False):
-    """Compile csrc/net_train.hip and csrc/doko_amd.hip for gfx950 and link them in the package directory
-    (in-tree).  profiling=True builds the phase-timer variant libdoko_amd_prof.so."""
+    """Compile csrc/doko_amd.hip and csrc/net_train.hip for gfx950, side by side, and link them in the package
+    directory (in-tree).  profiling=True builds the phase-timer variant libdoko_amd_prof.so."""
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     out = PROF_LIB_PATH if profiling else LIB_PATH
     with tempfile.TemporaryDirectory() as tmp:
-        obj = os.path.join(tmp, "net_train.o")
-        for cmd in ([hipcc] + TRAIN_FLAGS + ["-c", "-o", obj, TRAIN_SRC],
-                    [hipcc] + HIPCC_FLAGS + (["-DDK_PHASE_PROF"] if profiling else []) + ["-o", out, SRC, obj]):
-            if verbose:
-                print(" ".join(cmd))
-            subprocess.run(cmd, check=True, cwd=PKG_DIR)
+        objs = [os.path.join(tmp, "%d.o" % i) for i in range(len(UNITS))]
+        cmds = [[hipcc] + ARCH_FLAGS + flags + (["-DDK_PHASE_PROF"] if profiling else []) + ["-c", "-o", obj, src]
+                for (src, flags), obj in zip(UNITS, objs)]
+        link = [hipcc, "--offload-arch=gfx950", "-shared", "-o", out] + objs
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds + [link]), flush=True)
+        running = [subprocess.Popen(c, cwd=PKG_DIR) for c in cmds]
+        for p, c in zip(running, cmds):
+            if p.wait() != 0:
+                for q in running:
+                    q.wait()
+                raise subprocess.CalledProcessError(p.returncode, c)
+        subprocess.run(link, check=True, cwd=PKG_DIR)
     return out
-
-
-class dk_config(ctypes.Structure):
-    _fields_ = [("device", ctypes.c_int32), ("max_roots", ctypes.c_uint32),
-                ("max_iterations", ctypes.c_uint32), ("slot_capacity", ctypes.c_uint32)]
 
 
 class dk_net_adamw_tensor(ctypes.Structure):

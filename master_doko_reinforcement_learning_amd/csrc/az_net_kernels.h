@@ -998,7 +998,7 @@ __device__ __forceinline__ float gelu_erf(float v) {
     return v * phi;
 }
 
-// the same on a pair, so that the FMAs / multiplies issue as packed f32 (v_pk_fma_f32)
+// the same on a pair (the library is built without packed f32 instructions: two of each operation)
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2_t gelu_erf2(f32x2_t v) {
     const f32x2_t z = __builtin_elementwise_abs(v) * 0.70710678118654752f;
@@ -1168,8 +1168,8 @@ __device__ __forceinline__ float gelu_poly(float v) {
     return fmaf(-fabsf(v), fabsf(v) > 5.5f ? 0.0f : e, fmaxf(v, 0.0f));
 }
 
-// gelu_poly on a pair, its fma chain on packed f32 (v_pk_fma_f32: two lanes' values per
-// instruction), the same operations per element: bit-identical to two gelu_poly calls.
+// gelu_poly on a pair, the same operations per element: bit-identical to two gelu_poly calls (built without
+// packed f32 instructions, two of each).
 __device__ __forceinline__ f32x2_t gelu_poly_pk(f32x2_t v) {
     const float a0 = fminf(fabsf(v.x), 5.5f), a1 = fminf(fabsf(v.y), 5.5f);
     const f32x2_t a = {a0, a1};

@@ -2,7 +2,7 @@
 source lines each block's instructions come from (the attribution behind
 profiles/r06/valu_by_phase.json).
 
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off --cuda-device-only -S \
+    hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops --cuda-device-only -S \
         -gline-tables-only -o doko_g.s master_doko_reinforcement_learning_amd/csrc/doko_amd.hip
     python tools/isa_blocks.py doko_g.s 'search_kernelIN2dk4FdoEELb0ENS1_8NodeHot8E' [--json out.json]
 

@@ -2,7 +2,7 @@
 // (mlp_ln_f32x3_kernel<160, 32, 4, true>: x normalised with the producer's row statistics, x and the
 // next statistics written, no h).  Compiles the kernel header alone (seconds, not the library's
 // minutes), so that -D variants of the header can be timed and compared:
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off [-DVARIANT...] -o tools/mlp_lab tools/mlp_lab.hip
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops [-DVARIANT...] -o tools/mlp_lab tools/mlp_lab.hip
 //   tools/mlp_lab [rows] [reps] [dump-file]
 // Prints one JSON line: median / min kernel ms (HIP events, one launch each), the FNV-1a hash of
 // the outputs (x and the statistics: equal hashes = bit-identical results across variants), and in

@@ -3,7 +3,7 @@
 // SIMD, and stamps s_memtime (shader clock) / s_memrealtime (100 MHz) around the loop.  Output:
 // one JSON line per (kind, waves) with cycles per wave-instruction per SIMD and the shader clock
 // the stamps imply.  Used to price the rollout's per-ply code (profiles/r06/valu_rates.json).
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -o tools/valu_rates tools/valu_rates.hip
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/valu_rates tools/valu_rates.hip
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
