@@ -45,6 +45,11 @@ def build(verbose=False, profiling=False):
     return out
 
 
+class dk_config(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int32), ("max_roots", ctypes.c_uint32),
+                ("max_iterations", ctypes.c_uint32), ("slot_capacity", ctypes.c_uint32)]
+
+
 class dk_net_adamw_tensor(ctypes.Structure):
     _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("n", ctypes.c_uint64), ("block", ctypes.c_uint64),
                 ("id", ctypes.c_uint64)]
