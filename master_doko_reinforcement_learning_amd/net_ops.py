@@ -6,6 +6,7 @@ dk_net_adamw_async; csrc/train_*_kernels.h) on torch's current stream of the ten
 first two are differentiable (once).  f32, bf16 and f16; sums and statistics are f32.  There is no CPU
 fallback.  DokoAzNet.loss / DokoImpiNet.loss are built on the first two, NetTrainer on all three.
 """
+import collections
 import itertools
 import math
 import operator
@@ -237,8 +238,8 @@ def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
     if mask is not None and (mask.device != logits.device or mask.dtype != torch.bool or mask.shape not in (logits.shape, logits.shape[-1:])):
         raise ValueError("token_logprobs: mask is bool on the logits' device, in their shape or [%d]" % logits.shape[-1])
     temperature = float(temperature)
-    if not (temperature >= 1e-6 and math.isfinite(temperature)):
-        raise ValueError("token_logprobs: temperature %r (at least 1e-6)" % (temperature,))
+    if not 1e-6 <= temperature <= 1e30:
+        raise ValueError("token_logprobs: temperature %r (1e-6 to 1e30)" % (temperature,))
     if not 0 <= top <= TOP_MAX:
         raise ValueError("token_logprobs: top %r (0 to %d)" % (top, TOP_MAX))
     if torch.is_grad_enabled() and logits.requires_grad:
@@ -264,7 +265,8 @@ class AdamW(torch.optim.Optimizer):
     A group's parameters share one dtype and device and are dense.  The states lie in flat buffers
     (`buffers`, one dict a group; each parameter at a multiple of 256 elements) and state[p] holds views of
     them; `step` counts on the device for each parameter, so step() may be captured into a graph
-    (lr as a float is captured as it is)."""
+    (lr as a float is captured as it is).  step() raises the parameters' version counters, by which the networks'
+    fused forwards notice new weights; the replay of a captured one does not."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False):
         if state_bits not in (8, 32):
@@ -272,6 +274,22 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights = state_bits, bool(master_weights)
         self.buffers, self._tables = [], []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def __getstate__(self):   # (a copy or a pickle, which knows no e4m3: the codes as bytes; the buffers are laid out anew)
+        state = super().__getstate__()
+        state["state"] = {p: {k: v.view(torch.uint8) if v.dtype == torch.float8_e4m3fn else v for k, v in st.items()}
+                          for p, st in state["state"].items()}
+        return {**state, "state_bits": self.state_bits, "master_weights": self.master_weights}
+
+    @torch.no_grad()
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        old, self.state, self.buffers, self._tables = self.state, collections.defaultdict(dict), [], []
+        for group in self.param_groups:
+            self._lay_out(group)
+            for p in group["params"]:
+                for k, v in self.state[p].items():
+                    v.copy_(old[p][k].view(v.dtype) if v.dtype == torch.float8_e4m3fn else old[p][k])
 
     @torch.no_grad()
     def add_param_group(self, group):
@@ -334,6 +352,8 @@ class AdamW(torch.optim.Optimizer):
     def _step_group(self, group, b, t):
         dtype, device = t["dtype"], t["device"]
         lr, d_lr = _hyper(group)
+        if d_lr is not None and d_lr.device != device:
+            raise ValueError("AdamW: lr lies on another device than its group")
         params, at = group["params"], None
         grads = list(map(_GRAD, params))
         if not all(map(operator.is_not, grads, itertools.repeat(None))):
