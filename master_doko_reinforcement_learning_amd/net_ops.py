@@ -249,8 +249,8 @@ def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
 
 
 # ------------------------------------------------------------------------------- AdamW
-_GRAD, _DTYPE, _DEVICE, _LAYOUT = (operator.attrgetter(k) for k in ("grad", "dtype", "device", "layout"))
-_DENSE, _PTR = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+_GRAD, _DTYPE = operator.attrgetter("grad"), operator.attrgetter("dtype")
+_DENSE, _PTR, _INDEX = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.get_device   # (-1 on the CPU)
 _ROW = np.dtype([("p", np.uint64), ("g", np.uint64), ("n", np.uint64), ("block", np.uint64), ("id", np.uint64)])
 
 
@@ -362,12 +362,15 @@ class AdamW(torch.optim.Optimizer):
             if not params:
                 return
         # (checked anew each step, in maps: a network has a hundred tensors, and the step takes 20 us on the GPU)
-        if set(map(_DTYPE, params)) != {dtype} or set(map(_DEVICE, params)) != {device} or not all(map(_DENSE, params)):
+        if set(map(_DTYPE, params)) != {dtype} or set(map(_INDEX, params)) != {device.index} or not all(map(_DENSE, params)):
             raise RuntimeError("AdamW: a parameter was moved, cast or restrided since the optimiser was made")
-        if set(map(_DTYPE, grads)) != {dtype} or set(map(_LAYOUT, grads)) != {torch.strided}:
-            raise ValueError("AdamW: gradients are dense and in the parameters' dtype")
-        if not all(map(_DENSE, grads)):
-            grads = [g.contiguous() for g in grads]
+        try:
+            if set(map(_DTYPE, grads)) != {dtype}:
+                raise RuntimeError
+            if not all(map(_DENSE, grads)):   # (raises for a sparse one)
+                grads = [g.contiguous() for g in grads]
+        except RuntimeError:
+            raise ValueError("AdamW: gradients are dense and in the parameters' dtype") from None
         versions = t["versions"]
         if versions is not None:
             for i, p in zip(at or range(len(params)), params):
