@@ -26,7 +26,8 @@ _NET_OPS = {"layer_norm": "net_ops", "token_logprobs": "net_ops", "TokenLogprobs
 def __getattr__(name):
     if name in _NET_OPS:
         import importlib
-        return getattr(importlib.import_module("." + _NET_OPS[name], __name__), name)
+        globals()[name] = getattr(importlib.import_module("." + _NET_OPS[name], __name__), name)
+        return globals()[name]
     raise AttributeError("module %r has no attribute %r" % (__name__, name))
 
 

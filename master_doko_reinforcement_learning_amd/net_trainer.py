@@ -22,7 +22,9 @@ class NetTrainer:
     def step(self, *batch, **kwargs):
         """One step on net.loss(*batch, **kwargs); returns the loss before it (on the device, not synchronised)."""
         self.optimizer.zero_grad(set_to_none=True)
-        with torch.enable_grad():
+        # (the backward pass on this thread, not on the engine's for the GPU: without the hand-over of every step a
+        # batch of 64 positions takes 4.1 ms instead of 4.7, IMPI network)
+        with torch.enable_grad(), torch.autograd.set_multithreading_enabled(False):
             loss = self.net.loss(*batch, **kwargs)
             loss.backward()
         self.optimizer.step()
