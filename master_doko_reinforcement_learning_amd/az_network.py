@@ -1,4 +1,4 @@
-"""The AlphaZero policy/value network for full Doppelkopf, inference side.
+"""The AlphaZero policy/value network for full Doppelkopf: inference, and a differentiable forward with its loss.
 
 Architecture of rs-doko-py-bridge/python/az_doko.py:28-138 (AlphaZeroTicTacToeNetwork
 with TransformerBlock.py / SelfAttention.py), default config n_embd 160, 4 heads,

@@ -1,4 +1,4 @@
-"""The IMPI (autoregressive determinization) network, inference side.
+"""The IMPI (autoregressive determinization) network: inference, and a differentiable forward with its loss.
 
 Architecture of ImperfectInformationNetwork (rs-doko-py-bridge/python/main.py:99-138, with
 TransformerBlock.py / SelfAttention.py; PerClassAttentionMLPHead :25-55).  The configuration
