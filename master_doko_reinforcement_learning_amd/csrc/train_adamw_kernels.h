@@ -162,7 +162,10 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwTable tab, AdamwArgs a)
             r[j] *= sr.inverse;
             r[j] = r[j] > 0.0f ? fmaxf(r[j], 0x1p-9f) : r[j];
         }
-        // (behind the tensor's end gradient and moments are 0, and stay so: their codes are written as they were)
+        if (left < 4)   // what lies behind the tensor's end stays 0, also under a scale that is not finite
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (j >= left) m[j] = r[j] = 0.0f;
         ((uint32_t*)a.m)[q / 4] = f32_to_codes(m);
         ((uint32_t*)a.v)[q / 4] = f32_to_codes(r);
         if (lane == 0) {

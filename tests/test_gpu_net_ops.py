@@ -608,6 +608,13 @@ def test_adamw_special_gradients(bits):
     p.grad = torch.zeros(1024, device=DEV)
     opt.step()
     assert p[:512].isfinite().all()                      # 8 bits: a scale that is not finite is its own block's alone
+    q = torch.ones(300, device=DEV, requires_grad=True)  # a block that the tensor does not fill: nothing behind its end
+    opt = AdamW([q], state_bits=bits)
+    q.grad = torch.full((300,), math.inf, device=DEV)
+    for _ in range(2):
+        opt.step()
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert not opt.buffers[0][k][300:].float().any()
 
 
 def test_adamw_small_roots_are_kept():
