@@ -104,22 +104,26 @@ void with_small_vocab(uint32_t vocab, F f) {
 // a vocabulary worth their selection are wanted (20000 x 400 f32: 23 us against 24 for 5 of them, 56 against 25
 // for 20); by a wave each up to 1024 entries (20000 x 1000 bf16: 20 us, 63 with a workgroup each), and up to LOGP_WAVE
 // where the rows fill the GPU (4096 x 3000 bf16: 9 us against 14; 2048 x 20000: 32 against 24); else by a
-// workgroup each, or, where the rows are too few, in parts of at least 2 vectors a thread, a workgroup each.
+// workgroup each, or, where the rows are too few, in parts of at least 2 vectors a thread, a workgroup each.  Up to
+// a row for each CU, without alternatives, a workgroup of 16 waves takes a row up to LOGP_WIDE entries in one launch
+// (1 x 20000 f32: 5.5 us against 7.4 in parts; 200 x 20000: 6.9 against 8.5; 1 x 131072: 11.9 against 7.2).
 // The backward pass takes parts of 4 vectors a thread, a wave's up to LOGP_WAVE entries (20000 x 1000 bf16: 27 us
 // against 49; 20000 x 8000 f32: 248 against 267), beyond that a workgroup's (20000 x 20000 bf16: 333 against 362).
-constexpr uint32_t LOGP_SMALL = 512, LOGP_WAVE = 8192, LOGP_FILL = 1024, LOGP_GRID = 1u << 20;
+constexpr uint32_t LOGP_SMALL = 512, LOGP_WAVE = 8192, LOGP_WIDE = 65536, LOGP_WIDE_ROWS = 256, LOGP_FILL = 1024,
+                   LOGP_GRID = 1u << 20;
 bool logp_small(uint32_t vocab, uint32_t top) { return vocab <= LOGP_SMALL && (vocab <= 128 || top <= 8); }
-struct LogpPlan { bool small, wave; uint32_t splits, elems; };
+struct LogpPlan { bool small, wave, wide; uint32_t splits, elems; };
 LogpPlan logp_plan(uint64_t rows, uint32_t vocab, int type, uint32_t top) {
-    if (logp_small(vocab, top)) return {true, false, 1u, vocab};
+    if (logp_small(vocab, top)) return {true, false, false, 1u, vocab};
     const uint32_t unit = 256u * (type == DK_F32 ? 4u : 8u);   // a vector a thread
     const uint32_t units = (vocab + unit - 1) / unit;
     const bool wave = vocab <= 1024 || (rows >= 2048 && vocab <= LOGP_WAVE);
-    if (wave || rows >= LOGP_FILL) return {false, wave, 1u, units * unit};
+    if (top == 0 && !wave && rows <= LOGP_WIDE_ROWS && vocab <= LOGP_WIDE) return {false, false, true, 1u, units * unit};
+    if (wave || rows >= LOGP_FILL) return {false, wave, false, 1u, units * unit};
     const uint64_t want = LOGP_FILL / (rows ? rows : 1);
     uint32_t each = (uint32_t)((units + want - 1) / want);
     each = each < 2 ? 2 : each;
-    return {false, false, (units + each - 1) / each, each * unit};
+    return {false, false, false, (units + each - 1) / each, each * unit};
 }
 uint32_t logp_grid(uint64_t jobs) { return (uint32_t)(jobs < LOGP_GRID ? jobs : LOGP_GRID); }
 
@@ -215,6 +219,7 @@ int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t ro
         const dim3 grid(logp_grid(plan.wave ? (rows + 3) / 4 : rows * plan.splits)), block(256);
         if (plan.wave && top) hipLaunchKernelGGL((token_logprobs_kernel<T, WAVE, true>), grid, block, 0, st, a);
         else if (plan.wave) hipLaunchKernelGGL((token_logprobs_kernel<T, WAVE, false>), grid, block, 0, st, a);
+        else if (plan.wide) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, false>), grid, dim3(1024), 0, st, a);
         else if (top) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, true>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((token_logprobs_kernel<T, 256, false>), grid, block, 0, st, a);
         if (plan.splits > 1) hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3((uint32_t)rows), dim3(256), 0, st, a);

@@ -164,7 +164,8 @@ __global__ __launch_bounds__(256) void token_logprobs_small_kernel(LogpArgs a) {
     }
 }
 
-// W threads that share a row: a workgroup of 4 waves, or a wave
+// W threads that share a row: a workgroup of 4 or 16 waves, or a wave of a workgroup of 4
+constexpr int team_threads(int w) { return w > 256 ? w : 256; }
 template <int W>
 __device__ __forceinline__ void team_sync() {
     if constexpr (W > WAVE) __syncthreads();
@@ -182,8 +183,8 @@ __device__ __forceinline__ void team_sync() {
 template <int W>
 struct TopLds {
     static constexpr uint32_t ROOM = W > WAVE ? 1024 : 256;
-    uint64_t e[ROOM + 8], top[TOP_MAX], best[4];
-    uint32_t least[4], count, n_winners, winners[W];
+    uint64_t e[ROOM + 8], top[TOP_MAX], best[W / WAVE];
+    uint32_t least[W / WAVE], count, n_winners, winners[W];
 };
 template <int W, int BITS, class Scan, class Best>
 __device__ __forceinline__ void team_top(uint32_t k, uint32_t mine, TopLds<W>& lds, Scan scan, Best best) {
@@ -240,7 +241,7 @@ __device__ __forceinline__ void team_top(uint32_t k, uint32_t mine, TopLds<W>& l
     team_sync<W>();
 }
 
-// S and U of a team's threads together; `lds` has 4 entries
+// S and U of a team's threads together; `lds` has an entry for each wave
 template <int W>
 __device__ __forceinline__ Soft team_soft(Soft a, float c, Soft* lds) {
     a = lanes_soft<WAVE>(a, c);
@@ -287,9 +288,9 @@ __device__ __forceinline__ void load_logits(const T* x, const uint8_t* mask, uin
 // lie with the threads of the largest maxima: their elements alone are read again.  Without them (TOP false)
 // the kernel has half the registers: 103 us against 118.
 template <class T, int W, bool TOP>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(LogpArgs a) {
-    constexpr int V = VEC<T>, B = 16 / V, TEAMS = 256 / W;
-    __shared__ Soft soft_lds[4];
+__global__ __launch_bounds__(team_threads(W)) void token_logprobs_kernel(LogpArgs a) {
+    constexpr int V = VEC<T>, B = 16 / V, TEAMS = team_threads(W) / W;
+    __shared__ Soft soft_lds[team_threads(W) / WAVE];
     __shared__ TopLds<W> top_lds[TEAMS];
     TopLds<W>& lds = top_lds[threadIdx.x / W];
     const uint32_t tid = threadIdx.x % W;
