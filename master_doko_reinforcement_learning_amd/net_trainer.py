@@ -20,7 +20,10 @@ class NetTrainer:
         self.optimizer = AdamW(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits)
 
     def step(self, *batch, **kwargs):
-        """One step on net.loss(*batch, **kwargs); returns the loss before it (on the device, not synchronised)."""
+        """One step on net.loss(*batch, **kwargs); returns the loss before it (on the device, not synchronised).
+        Not to be captured into a graph: the library calls of the networks' heads and embeddings are not."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("NetTrainer.step is not captured into graphs (AdamW.step is)")
         self.optimizer.zero_grad(set_to_none=True)
         # (the backward pass on this thread, not on the engine's for the GPU: without the hand-over of every step a
         # batch of 64 positions takes 4.1 ms instead of 4.7, IMPI network)

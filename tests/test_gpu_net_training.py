@@ -82,7 +82,8 @@ def test_loss_and_gradients_are_as_exact_as_the_plain_modules(make):
     gg = _grads(got, net)
     size = _distance(gw, [torch.zeros_like(g) for g in gw])
     assert _distance(gg, gw) <= 2 * _distance(gp, gw) + 64 * ref.U * size
-    assert abs(float(got) - float(want)) <= 2 * abs(float(plain) - float(want)) + 64 * ref.U * abs(float(want))
+    got, plain, want = got.item(), plain.item(), want.item()
+    assert abs(got - want) <= 2 * abs(plain - want) + 64 * ref.U * abs(want)
     # the forwards agree as closely
     with torch.no_grad():
         a, b = net.forward_train(batch[0]), net.forward_torch(batch[0])
@@ -173,3 +174,13 @@ def test_trainer_refuses():
         NetTrainer(net)
     with pytest.raises(ValueError):
         NetTrainer(net.to(DEV).bfloat16())
+    net, batch = _impi(d=32)
+    trainer, batch = NetTrainer(net.to(DEV)), tuple(t.to(DEV) for t in batch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        two = torch.ones(1, device=DEV) + 1
+        with pytest.raises(RuntimeError):
+            trainer.step(*batch)
+    graph.replay()
+    assert float(two) == 2
+    trainer.step(*batch)
