@@ -110,7 +110,7 @@ void with_small_vocab(uint32_t vocab, F f) {
 // The backward pass takes parts of 4 vectors a thread, a wave's up to LOGP_WAVE entries (20000 x 1000 bf16: 27 us
 // against 49; 20000 x 8000 f32: 248 against 267), beyond that a workgroup's (20000 x 20000 bf16: 333 against 362).
 constexpr uint32_t LOGP_SMALL = 512, LOGP_WAVE = 8192, LOGP_WIDE = 65536, LOGP_WIDE_ROWS = 256, LOGP_FILL = 1024,
-                   LOGP_GRID = 1u << 20;
+                   LOGP_GROUPED = 16384, LOGP_GRID = 1u << 20;
 bool logp_small(uint32_t vocab, uint32_t top) { return vocab <= LOGP_SMALL && (vocab <= 128 || top <= 8); }
 struct LogpPlan { bool small, wave, wide; uint32_t splits, elems; };
 LogpPlan logp_plan(uint64_t rows, uint32_t vocab, int type, uint32_t top) {
@@ -217,11 +217,12 @@ int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t ro
             return;
         }
         const dim3 grid(logp_grid(plan.wave ? (rows + 3) / 4 : rows * plan.splits)), block(256);
-        if (plan.wave && top) hipLaunchKernelGGL((token_logprobs_kernel<T, WAVE, true>), grid, block, 0, st, a);
-        else if (plan.wave) hipLaunchKernelGGL((token_logprobs_kernel<T, WAVE, false>), grid, block, 0, st, a);
-        else if (plan.wide) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, false>), grid, dim3(1024), 0, st, a);
-        else if (top) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((token_logprobs_kernel<T, 256, false>), grid, block, 0, st, a);
+        if (plan.wave && top) hipLaunchKernelGGL((token_logprobs_kernel<T, WAVE, 1>), grid, block, 0, st, a);
+        else if (plan.wave) hipLaunchKernelGGL((token_logprobs_kernel<T, WAVE, 0>), grid, block, 0, st, a);
+        else if (plan.wide) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0>), grid, dim3(1024), 0, st, a);
+        else if (top && plan.elems >= LOGP_GROUPED) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 4>), grid, block, 0, st, a);
+        else if (top) hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 1>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((token_logprobs_kernel<T, 256, 0>), grid, block, 0, st, a);
         if (plan.splits > 1) hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3((uint32_t)rows), dim3(256), 0, st, a);
     });
     DK_HIP(hipGetLastError());

@@ -175,24 +175,27 @@ __device__ __forceinline__ void team_sync() {
     }
 }
 
-// The k largest of a team's entries, sorted, in lds.top[0 .. k) (0 behind the last).  `mine` is the largest
-// key among a thread's entries; scan(least, push) goes through the entries of the threads whose mine is at
-// least `least` and pushes those whose key is; best(below) is the thread's largest entry under `below`.
-//   Of a wave's threads at least k have mine >= T for the k-th largest T of them, so no entry below any
+// The k largest of a team's entries, sorted, in lds.top[0 .. k) (0 behind the last).  A thread's entries come in
+// S groups, mine[s] is the largest key of a group; scan(least, push) goes through the groups whose mine is at
+// least `least` and pushes the entries whose key is; best(below) is the thread's largest entry under `below`.
+//   Of a wave's groups at least k have mine >= T for the k-th largest T of them, so no entry below any
 // wave's T is among the k largest: the others are few, except where many are equal.
-template <int W>
+template <int W, int S>
 struct TopLds {
     static constexpr uint32_t ROOM = W > WAVE ? 1024 : 256;
     uint64_t e[ROOM + 8], top[TOP_MAX], best[W / WAVE];
-    uint32_t least[W / WAVE], count, n_winners, winners[W];
+    uint32_t least[W / WAVE], count, n_winners, winners[S * W], keys[S][W];
 };
-template <int W, int BITS, class Scan, class Best>
-__device__ __forceinline__ void team_top(uint32_t k, uint32_t mine, TopLds<W>& lds, Scan scan, Best best) {
+template <int W, int BITS, int S, class Scan, class Best>
+__device__ __forceinline__ void team_top(uint32_t k, const uint32_t (&mine)[S], TopLds<W, S>& lds, Scan scan, Best best) {
     const uint32_t tid = threadIdx.x % W;
     uint32_t least = 0;
     for (int b = 31; b >= 32 - BITS; --b) {
         const uint32_t next = least | 1u << b;
-        if ((uint32_t)__popcll(__ballot(mine >= next)) >= k) least = next;
+        uint32_t n = 0;
+#pragma unroll
+        for (int g = 0; g < S; ++g) n += (uint32_t)__popcll(__ballot(mine[g] >= next));
+        if (n >= k) least = next;
     }
     if constexpr (W > WAVE) {
         if (tid % WAVE == 0) lds.least[tid / WAVE] = least;
@@ -204,11 +207,11 @@ __device__ __forceinline__ void team_top(uint32_t k, uint32_t mine, TopLds<W>& l
     if (least == 0) least = 1;
     scan(least, [&](uint32_t key, uint32_t index) {
         const uint32_t at = atomicAdd(&lds.count, 1u);   // (any order: the ranks below depend on the set alone)
-        if (at < TopLds<W>::ROOM) lds.e[at] = entry(key, index);
+        if (at < TopLds<W, S>::ROOM) lds.e[at] = entry(key, index);
     });
     team_sync<W>();
     const uint32_t count = lds.count;
-    if (count <= TopLds<W>::ROOM) {
+    if (count <= TopLds<W, S>::ROOM) {
         if (tid < 8) lds.e[count + tid] = 0;   // (whole groups of 8 below)
         team_sync<W>();
         for (uint32_t i = tid; i < count; i += W) {
@@ -284,15 +287,18 @@ __device__ __forceinline__ void load_logits(const T* x, const uint8_t* mask, uin
 
 // Larger vocabularies: W threads go once through a row, or a workgroup through one of its `splits` parts
 // where the rows are too few to fill the GPU, each thread with a running maximum (rebased every 16 elements:
-// 4096 x 65536 bf16 takes 103 us so, 5.2 TB/s, 107 us with 32, whose registers cost waves).  The top entries
-// lie with the threads of the largest maxima: their elements alone are read again.  Without them (TOP false)
-// the kernel has half the registers: 103 us against 118.
-template <class T, int W, bool TOP>
+// 4096 x 65536 bf16 takes 99 us so, 5.4 TB/s, 107 us with 32, whose registers cost waves).  The top entries
+// lie with the largest of the threads' maxima, of which there is one for each of GROUPS groups of a thread's
+// elements: the groups of the largest are read again.  4 groups where a workgroup reads 16384 entries or more (1500 x
+// 131072 f32 with 20 alternatives: 183 us against 251 with one), else one (20000 x 9000 f16: 159 us against 178).
+// Without alternatives (GROUPS 0) the kernel has half the registers: 99 us against 118.
+template <class T, int W, int GROUPS>
 __global__ __launch_bounds__(team_threads(W)) void token_logprobs_kernel(LogpArgs a) {
+    constexpr bool TOP = GROUPS > 0;
     constexpr int V = VEC<T>, B = 16 / V, TEAMS = team_threads(W) / W;
     __shared__ Soft soft_lds[team_threads(W) / WAVE];
-    __shared__ TopLds<W> top_lds[TEAMS];
-    TopLds<W>& lds = top_lds[threadIdx.x / W];
+    __shared__ TopLds<W, TOP ? GROUPS : 1> top_lds[TEAMS];
+    auto& lds = top_lds[threadIdx.x / W];
     const uint32_t tid = threadIdx.x % W;
     const float c = a.inv_t * LOG2E;
     const uint64_t jobs = a.rows * a.splits;
@@ -306,10 +312,13 @@ __global__ __launch_bounds__(team_threads(W)) void token_logprobs_kernel(LogpArg
         Token token{};
         if (a.splits == 1) token = load_token<T>(a, row, tid);   // (at most 64 tokens)
         Soft mine{LOWEST, 0.0f, 0.0f};
+        float seen = NEG_INF;   // the largest element of the present group
         auto take = [&](const float* v, int n) {
-            float m = mine.m;
+            float most = v[0];
 #pragma unroll
-            for (int j = 0; j < n; ++j) m = fmaxf(m, v[j]);
+            for (int j = 1; j < n; ++j) most = fmaxf(most, v[j]);
+            if (TOP) seen = fmaxf(seen, most);
+            const float m = fmaxf(mine.m, most);
             mine = rebased(mine, m, c);
 #pragma unroll
             for (int j = 0; j < n; ++j) {
@@ -318,12 +327,28 @@ __global__ __launch_bounds__(team_threads(W)) void token_logprobs_kernel(LogpArg
                 mine.u += fmaxf(z, LOWEST) * e;
             }
         };
+        // a thread's elements in groups of whole batches, one after the other
+        constexpr uint32_t SHARE = (TOP ? GROUPS : 1) * B;
+        const uint32_t group = (rounds + SHARE - 1) / SHARE * B;   // vectors of one
+        uint32_t groups = 0, ahead = group;
         uint32_t first = lo;
         float v[B * V];
         for (; hi - first >= B * W * V; first += B * W * V) {
+            if (TOP && GROUPS > 1) {
+                if (ahead == 0) {
+                    lds.keys[groups++][tid] = order_key(seen);
+                    seen = NEG_INF;
+                    ahead = group;
+                }
+                ahead -= B;
+            }
 #pragma unroll
             for (int i = 0; i < B; ++i) load_logits<T, true>(x, mask, first + (i * W + tid) * V, hi, v + i * V);
             take(v, B * V);
+        }
+        if (TOP && GROUPS > 1 && ahead == 0 && first < hi) {
+            lds.keys[groups++][tid] = order_key(seen);
+            seen = NEG_INF;
         }
         // the rest, less than B vectors a thread: all loads first, then the sums of those that there are
 #pragma unroll
@@ -332,19 +357,24 @@ __global__ __launch_bounds__(team_threads(W)) void token_logprobs_kernel(LogpArg
 #pragma unroll
         for (int i = 0; i < B; ++i)
             if (first + (i * W + tid) * V < hi) take(v + i * V, V);
-        const uint32_t key = mine.s == 0.0f ? 0u : order_key(mine.m);
         const Soft all = team_soft<W>(mine, c, soft_lds);
-        if constexpr (TOP)
+        if constexpr (TOP) {
+            uint32_t key[GROUPS];
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) key[g] = (uint32_t)g < groups ? lds.keys[g][tid] : (uint32_t)g == groups ? order_key(seen) : 0u;
             team_top<W, KEY_BITS<T>>(
                 a.top, key, lds,
                 [&](uint32_t least, auto push) {
                     if (tid == 0) lds.n_winners = 0;
                     team_sync<W>();
-                    if (key >= least) lds.winners[atomicAdd(&lds.n_winners, 1u)] = tid;
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g)
+                        if (key[g] >= least) lds.winners[atomicAdd(&lds.n_winners, 1u)] = g * W + tid;
                     team_sync<W>();
-                    const uint32_t vectors = lds.n_winners * rounds;
+                    const uint32_t vectors = lds.n_winners * group;
                     for (uint32_t i = tid; i < vectors; i += W) {
-                        const uint32_t at = lo + (i % rounds * W + lds.winners[i / rounds]) * V;
+                        const uint32_t w = lds.winners[i / group], at = lo + ((w / W * group + i % group) * W + w % W) * V;
+                        if (at >= hi) continue;
                         float v[V];
                         load_logits<T, false>(x, mask, at, hi, v);
 #pragma unroll
@@ -368,6 +398,7 @@ __global__ __launch_bounds__(team_threads(W)) void token_logprobs_kernel(LogpArg
                     }
                     return best;
                 });
+        }
         if (a.splits == 1) {
             const RowSoft r = finish_row(all, a.inv_t);
             if (tid == 0) finish_stats(a, row, r);
@@ -385,15 +416,15 @@ __global__ __launch_bounds__(team_threads(W)) void token_logprobs_kernel(LogpArg
 template <class T>
 __global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogpArgs a) {
     __shared__ Soft soft_lds[4];
-    __shared__ TopLds<256> lds;
+    __shared__ TopLds<256, 1> lds;
     const uint64_t row = blockIdx.x;
     const float c = a.inv_t * LOG2E;
     const uint64_t* e = a.part_top + row * a.splits * a.top;
     const uint32_t n = a.splits * a.top;
-    uint32_t key = 0;
+    uint32_t key[1] = {0};
     for (uint32_t i = threadIdx.x; i < n; i += 256) {
         const uint32_t k = (uint32_t)(e[i] >> 32);
-        key = k > key ? k : key;
+        key[0] = k > key[0] ? k : key[0];
     }
     const Token token = load_token<T>(a, row, threadIdx.x);
     Soft mine{LOWEST, 0.0f, 0.0f};

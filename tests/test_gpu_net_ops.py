@@ -320,25 +320,45 @@ def test_token_logprobs_many_tokens(n, vocab):
     _logp_check(x, t, mask, None, de, top=2)
 
 
+def _tied_rows(vocab, g):
+    x = torch.zeros(8, vocab, device=DEV)
+    i = torch.arange(vocab, device=DEV)
+    x[1] = torch.randint(0, 3, (vocab,), generator=g, device=DEV).float()
+    x[2, vocab // 2:] = 1.0
+    x[3] = -0.0
+    x[3, ::2] = 0.0                                            # +0 and -0 are equal
+    x[4] = i / 64.0                                            # ascending: the best lie at the end
+    x[5] = -i / 64.0
+    x[6] = torch.where(i % 2048 < 16, 5.0, 0.0)                # large ones at a period
+    x[7] = torch.where(i % 2048 < 16, 5.0 + i / 1024.0, 0.0)
+    return x
+
+
 @pytest.mark.parametrize("vocab", [33, 1000, 1500, 70001])
 @pytest.mark.parametrize("top", [1, 7, 32])
 def test_token_logprobs_ties(vocab, top):
     """Equal logits: the lowest index first, wherever the equal ones lie."""
     g = _gen(vocab + top)
-    x = torch.zeros(8, vocab, device=DEV)
-    x[1] = torch.randint(0, 3, (vocab,), generator=g, device=DEV).float()
-    x[2, vocab // 2:] = 1.0
-    x[3] = -0.0
-    x[3, ::2] = 0.0                                            # +0 and -0 are equal
-    x[4] = torch.arange(vocab, device=DEV) / 64.0              # ascending: the best lie at the end
-    x[5] = -torch.arange(vocab, device=DEV) / 64.0
-    x[6] = torch.where(torch.arange(vocab, device=DEV) % 2048 < 16, 5.0, 0.0)    # large ones at a period
-    x[7] = torch.where(torch.arange(vocab, device=DEV) % 2048 < 16, 5.0 + torch.arange(vocab, device=DEV) / 1024.0, 0.0)
+    x = _tied_rows(vocab, g)
     t = torch.zeros(8, 1, dtype=torch.int64, device=DEV)
     for dtype in (F32, BF16):
         _logp_check(x.to(dtype), t, None, None, None, top=top)
     mask = torch.rand(8, vocab, generator=g, device=DEV) < 0.5
     _logp_check(x, t, mask, None, None, top=top)
+
+
+@pytest.mark.parametrize("vocab,rows", [(300, 64), (900, 2048), (3000, 2048), (9001, 1032), (17001, 1032), (33001, 1032)])
+@pytest.mark.parametrize("top", [3, 32])
+def test_token_logprobs_ties_in_many_rows(vocab, rows, top):
+    """The same where the rows fill the GPU, with the rows' order mixed and a mask that leaves some of them little."""
+    g = _gen(vocab + top)
+    x = _tied_rows(vocab, g).repeat(rows // 8, 1)[torch.randperm(rows, generator=g, device=DEV)]
+    t = torch.randint(0, vocab, (rows, 2), generator=g, device=DEV)
+    for dtype in (F32, BF16):
+        _logp_check(x.to(dtype), t, None, None, None, top=top)
+    share = torch.rand(rows, 1, generator=g, device=DEV) ** 8     # from nothing to nearly all
+    mask = torch.rand(rows, vocab, generator=g, device=DEV) < share
+    _logp_check(x.to(F16), t, mask, None, None, top=top)
 
 
 @pytest.mark.parametrize("vocab", [39, 3000, 40000])
