@@ -628,7 +628,8 @@ int dk_net_attn62_bias_f32_async(const void* qkv, const void* bqkv, void* y, uin
  * What a training step of the networks chains (az_doko.py's fit: norm, loss, update).  Each call runs
  * on the caller's stream, allocates and synchronises nothing and may be captured into a graph.  Element
  * types are dk_net_type; every sum and statistic is f32.  Strides are in elements between rows; the
- * last dimension is dense and rows need no alignment beyond their elements'. */
+ * last dimension is dense and rows need no alignment beyond their elements'.  Statistics, workspaces and
+ * AdamW's states begin at multiples of 16 bytes. */
 enum dk_net_type { DK_F32 = 0, DK_BF16 = 1, DK_F16 = 2 };
 
 /* dk_net_layer_norm_async: x_out = x + delta (rounded to `type`), h_out = LayerNorm(x_out; gamma, beta,

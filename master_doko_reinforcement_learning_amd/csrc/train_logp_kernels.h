@@ -17,7 +17,7 @@
 namespace dk {
 namespace train {
 
-constexpr float NEG_INF = -__builtin_huge_valf(), LOWEST = -3.40282347e+38f, LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+constexpr float NEG_INF = -__builtin_huge_valf(), LOWEST = -3.40282347e+38f, LOG2E = 1.44269504088896341f;
 constexpr uint32_t TOP_MAX = 32, TOKENS_MAX = 64;
 
 // a logit's order as an unsigned key: larger key = larger value, +0 and -0 the same; 0 for what is
@@ -129,7 +129,10 @@ __global__ __launch_bounds__(256) void token_logprobs_small_kernel(LogpArgs a) {
                 if (at < a.vocab && !mask[at]) v[i] = NEG_INF;
             }
         }
-        const Token token = load_token<T>(a, row, lane);
+        constexpr int Q = TOKENS_MAX / G;
+        Token token[Q];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) token[i] = load_token<T>(a, row, lane + i * G);
         float m = LOWEST;
 #pragma unroll
         for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
@@ -143,7 +146,8 @@ __global__ __launch_bounds__(256) void token_logprobs_small_kernel(LogpArgs a) {
         }
         const RowSoft r = finish_row({m, lanes_reduce<G, Add>(s), lanes_reduce<G, Add>(u)}, a.inv_t);
         if (lane == 0) finish_stats(a, row, r);
-        for (uint32_t i = lane; i < a.n; i += G) finish_token(a, row, i, i == lane ? token : load_token<T>(a, row, i), r);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) finish_token(a, row, lane + i * G, token[i], r);
         if (a.top == 0) continue;
         uint32_t key[E];
 #pragma unroll

@@ -84,6 +84,11 @@ def test_layer_norm_rows(rows, d, dtype):
     _norm_check(*_norm_case(rows, d, dtype, dtype, rows, residual=rows % 2 == 0))
 
 
+@pytest.mark.parametrize("rows,d,dtype", [(140009, 33, F32), (70001, 250, F16), (40009, 160, BF16), (33001, 500, F32), (9001, 1500, BF16)])
+def test_layer_norm_more_rows_than_the_grid_holds(rows, d, dtype):
+    _norm_check(*_norm_case(rows, d, dtype, F32, rows, residual=rows % 2 == 0))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("d", [1, 5, 160, 257, 1024, 3001, 9001])
 @pytest.mark.parametrize("pad", [1, 7, 64])
@@ -469,6 +474,25 @@ def test_token_logprobs_gradient_against_differences():
     slope, want = (total[0] - total[1]) / (2 * step), float((dx.double() * v.double()).sum())
     # 24 values of magnitude <= ~8, off by 100 u each; third derivatives of lse and entropy along v are at most ~40 |v|^3 a term
     assert abs(slope - want) <= 24 * 8 * 100 * ref.U / step + step ** 2 / 6 * 24 * 40
+
+
+@pytest.mark.parametrize("rows,vocab", [(17000003, 3), (4200003, 100), (4200003, 530)])
+def test_token_logprobs_more_rows_than_the_grid_holds(rows, vocab):
+    from master_doko_reinforcement_learning_amd import token_logprobs
+    x = torch.zeros(rows, vocab, dtype=BF16, device=DEV)
+    x[-9:] = _randn(_gen(1), 9, vocab, dtype=BF16, scale=3.0)
+    x.requires_grad_()
+    t = torch.full((rows,), vocab - 1, device=DEV)
+    dl = torch.zeros(rows, device=DEV)
+    dl[-9:] = 1.0
+    got = token_logprobs(x, t, top=2)
+    dx, = torch.autograd.grad(got.logprobs, x, dl)
+    tail = x.detach()[-9:]
+    want, _, _ = ref.logp(tail.double(), t[-9:, None], None, 1.0, dl[-9:, None].double(), None, BF16)
+    assert ref.off(got.logprobs.detach()[-9:, None], *want["logprobs"]) <= 1 and ref.off(got.entropy.detach()[-9:], *want["entropy"]) <= 1
+    assert torch.equal(got.top_tokens[-9:], _tops(tail, None, 2)[1]) and (got.top_tokens[:-9] == torch.arange(2, device=DEV)).all()
+    assert ref.off(dx[-9:], *want["dlogits"]) <= 1 and not dx[:-9].any()
+    assert (got.logprobs.detach()[:-9] + math.log(vocab)).abs().max() <= 8 * ref.U * (math.log(vocab) + 1)
 
 
 def test_token_logprobs_past_32_bits():

@@ -78,3 +78,23 @@ def test_adamw_entry_refuses():
                 dict(b1=float("nan")), dict(eps=-1.0), dict(rows=((None, p, 8, 0, 0),)), dict(rows=((p, None, 8, 0, 0),)), dict(rows=((p, p, 1 << 50, 0, 0),))):
         assert step(**bad) == INVALID, bad
     assert step(rows=()) == 0
+
+
+def test_launches_go_to_the_tensors_device(monkeypatch):
+    """A tensor on another device than the current one: its device is current during the call, and the stream is its own."""
+    import contextlib
+
+    from master_doko_reinforcement_learning_amd import net_ops
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(index):
+        current.append(index)
+        yield
+        current.pop()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[-1])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(net_ops, "_raw_stream", lambda i: 100 + i)
+    entry = lambda *a: seen.append((current[-1],) + a) or 0  # noqa: E731
+    assert net_ops._launch(entry, 0, "x") == 0 and net_ops._launch(entry, 3, "y") == 0
+    assert seen == [(0, "x", 100), (3, "y", 103)] and current == [0]
