@@ -659,7 +659,7 @@ int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* 
  *   stats [rows][2]       the largest allowed logit and log sum e^(z - its z), for the backward pass (NULL: not wanted)
  *   top_logprobs, top_tokens [rows][top]   the largest by (logit descending, index ascending); where fewer are
  *                         allowed -inf and -1
- * n <= 64, top <= 32.  A row with nothing allowed has entropy 0.  Whatever a masked entry
+ * n <= 64, top <= 32, temperature 1e-6 to 1e30.  A row with nothing allowed has entropy 0.  Whatever a masked entry
  * holds is not looked at; a NaN or +inf in an allowed one makes the row's floating results NaN (its
  * top_tokens are still tokens of the row, NaN never among them).
  * mask_stride 0 applies one mask to every row.  The workspace has dk_net_token_logprobs_workspace bytes
@@ -680,7 +680,7 @@ int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_
 
 /* dk_net_adamw_async: one AdamW step of `count` tensors (host array; dense parameters and gradients of
  * `type`).  A tensor's states are the blocks of 256 elements from `block` on in the flat buffers; no block
- * belongs to two tensors.  state_bits 32: exp_avg / exp_avg_sq are f32.  state_bits 8: e4m3 codes of exp_avg
+ * or id belongs to two tensors, and the tensors' memory does not overlap.  state_bits 32: exp_avg / exp_avg_sq are f32.  state_bits 8: e4m3 codes of exp_avg
  * and of sqrt(exp_avg_sq), times one f32 scale for each block.  master (or NULL): f32 weights laid out as the states;
  * the step is theirs and p receives them rounded.  step (int32) and factors (3 floats, scratch) are indexed
  * by `id`: step[id] counts on the device, so that a captured step goes on counting.  d_lr (or NULL) is

@@ -37,6 +37,8 @@ void with_type(int type, F f) {
     else if (type == DK_BF16) f(__bf16{});
     else f(_Float16{});
 }
+// (what lies outside would overflow in f32, as the reciprocal or in sums of differences of logits)
+bool temperature_ok(float t) { return t >= 1e-6f && t <= 1e30f; }
 // the same for a weight: f32, or the activations' type T
 template <class T, class F>
 void with_weight(int wtype, F f) {
@@ -194,7 +196,7 @@ int dk_net_token_logprobs_async(const void* logits, uint64_t stride, uint64_t ro
                                 uint32_t n, uint32_t top, float* logprobs, float* entropy, float* stats, float* top_logprobs,
                                 int64_t* top_tokens, void* workspace, uint64_t workspace_bytes, void* stream) {
     if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || top > TOP_MAX || rows > MAX_ROWS ||
-        !(temperature > 0.0f) || std::isinf(temperature))
+        !temperature_ok(temperature))
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
     if (!logits || (n && (!tokens || !logprobs)) || (top && (!top_logprobs || !top_tokens))) return DK_E_INVALID;
@@ -240,8 +242,8 @@ int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_
                                     const uint8_t* mask, uint64_t mask_stride, float temperature, const int64_t* tokens,
                                     uint32_t n, const float* logprobs, const float* stats, const float* entropy,
                                     const float* dlogprobs, const float* dentropy, void* dlogits, void* stream) {
-    if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || rows > MAX_ROWS || !(temperature > 0.0f) ||
-        std::isinf(temperature))
+    if (!type_ok(type) || vocab == 0 || vocab > 0x7FFFFFFFu || n > TOKENS_MAX || rows > MAX_ROWS ||
+        !temperature_ok(temperature))
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
     if (!logits || (n && (!tokens || !logprobs)) || !stats || !entropy || !dlogits) return DK_E_INVALID;

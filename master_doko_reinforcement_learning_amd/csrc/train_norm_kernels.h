@@ -23,6 +23,9 @@ namespace train {
 template <int LANES_, int NV_>
 struct NormShape {
     static constexpr int LANES = LANES_, NV = NV_, THREADS = LANES_ > 256 ? LANES_ : 256, ROWS = THREADS / LANES_;
+    // whether column c + j of vector i lies in a row of d: only the last vector can reach behind it, as with one
+    // vector less a row would not fit
+    static __device__ __forceinline__ bool inside(int i, uint32_t c, uint32_t d) { return i + 1 < NV_ || c < d; }
     // whether the next row is loaded under the present one's reductions: where registers are left for it
     template <class T>
     static constexpr bool AHEAD = NV_ * VEC<T> <= 16;
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(S::THREADS) void layer_norm_kernel(NormArgs a) {
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                v[i][j] = (t + i * L) * V + j < d ? v[i][j] - mu : 0.0f;
+                v[i][j] = S::inside(i, (t + i * L) * V + j, d) ? v[i][j] - mu : 0.0f;
                 sq += v[i][j] * v[i][j];
             }
         row_sum<L>(sq, none, lds, 1);
@@ -177,7 +180,7 @@ __global__ __launch_bounds__(S::THREADS) void layer_norm_bwd_kernel(NormBwdArgs 
     uint64_t row = (uint64_t)blockIdx.x * S::ROWS + threadIdx.x / L;
     Vec<T> xr[NV], gr[NV], res[NV];
     float2 st;
-    auto load = [&](uint64_t at) {   // (0 behind the row's end: such columns add nothing)
+    auto load = [&](uint64_t at) {   // (0 behind the row's end)
         at = at < last ? at : last;
         st = *(const float2*)(a.stats + 2 * at);
         load_row<T, NV, L>(a.x, a.xs, at, t, d, xr);
@@ -196,7 +199,7 @@ __global__ __launch_bounds__(S::THREADS) void layer_norm_bwd_kernel(NormBwdArgs 
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float g0 = live ? to_f32((T)gr[i][j]) : 0.0f;
-                n[i][j] = (to_f32((T)xr[i][j]) - mu) * r;
+                n[i][j] = S::inside(i, (t + i * L) * V + j, d) ? (to_f32((T)xr[i][j]) - mu) * r : 0.0f;
                 g[i][j] = g0 * w[i][j];
                 if (a.dres) e[i][j] = to_f32((T)res[i][j]);
                 sg += g[i][j];

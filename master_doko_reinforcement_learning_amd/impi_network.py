@@ -55,7 +55,7 @@ class DokoImpiNet(nn.Module):
 
     def loss(self, tokens, guesses, mask=None):
         """Mean cross entropy of the guesses [B] (ImperfectInformationOutput classes; negative: not counted) under
-        the consistent classes `mask` [B, 33]."""
+        the consistent classes `mask` [B, 33] (infinite where a guess is not among them)."""
         from .net_ops import token_logprobs
         lp = token_logprobs(self.forward_train(tokens), guesses, mask=mask).logprobs
         return -lp.sum() / (guesses >= 0).sum().clamp(min=1)

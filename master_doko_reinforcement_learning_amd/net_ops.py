@@ -222,7 +222,7 @@ def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
     logits [..., vocab]; tokens int64 or int32 [...] or [..., n] with n <= 64; a negative one is padding (log
     probability 0, no gradient), one >= vocab gives NaN and no gradient.  mask: bool [..., vocab] or [vocab],
     True for what is allowed; a token that is not has log probability -inf and no gradient, and what a masked
-    logit holds is not looked at.  A row with nothing allowed has entropy 0.  Alternatives are ordered by
+    logit holds is not looked at (nor has one a gradient whose log probability is below float32's range).  A row with nothing allowed has entropy 0.  Alternatives are ordered by
     logit, equal ones by index; -1 (and -inf) behind the last allowed one."""
     _floating(logits, "token_logprobs")
     if logits.dim() == 0 or logits.shape[-1] == 0:
@@ -262,7 +262,7 @@ class AdamW(torch.optim.Optimizer):
     f32 weights that the optimiser keeps; a parameter that was written to since the last step (a loaded
     state_dict) is taken over into its master first.  lr may be a one-element f32 tensor on the GPU.
 
-    A group's parameters share one dtype and device and are dense.  The states lie in flat buffers
+    A group's parameters share one dtype and device, are dense and do not overlap.  The states lie in flat buffers
     (`buffers`, one dict a group; each parameter at a multiple of 256 elements) and state[p] holds views of
     them; `step` counts on the device for each parameter, so step() may be captured into a graph
     (lr as a float is captured as it is).  step() raises the parameters' version counters, by which the networks'
@@ -307,6 +307,9 @@ class AdamW(torch.optim.Optimizer):
             _floating(p, "AdamW")
             if p.dtype != params[0].dtype or p.device != params[0].device or not p.is_contiguous():
                 raise ValueError("AdamW: a group's parameters are dense and share one dtype and device")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):   # (they are updated side by side)
+            raise ValueError("AdamW: a group's parameters overlap, or one is given twice")
         master = self.master_weights and bool(params) and params[0].dtype != torch.float32
         dev = params[0].device if params else None
         table = np.zeros(len(params), _ROW)
@@ -398,6 +401,8 @@ class AdamW(torch.optim.Optimizer):
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the state_dict has other parameter groups")
+        if any(g.get("amsgrad") or g.get("maximize") for g in groups):
+            raise ValueError("AdamW: the state_dict is of another update (amsgrad, maximize)")
         todo = []
         for mine, theirs in zip(self.param_groups, groups):
             for p, key in zip(mine["params"], theirs["params"]):
@@ -412,7 +417,11 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError("AdamW: the state_dict's %s does not fit (state_bits %d)" % (k, self.state_bits))
                     todo.append((own, v))
         for mine, theirs in zip(self.param_groups, groups):
-            mine.update({k: v for k, v in theirs.items() if k in self.defaults})
+            lr = mine["lr"]
+            mine.update({k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in theirs.items() if k != "params"})
+            if isinstance(lr, torch.Tensor):   # (a captured step reads it)
+                lr.copy_(torch.as_tensor(mine["lr"]).reshape(lr.shape))
+                mine["lr"] = lr
         for own, v in todo:
             if v is None:
                 own.view(torch.uint8 if own.dtype == torch.float8_e4m3fn else own.dtype).zero_()

@@ -210,6 +210,24 @@ def test_layer_norm_far_from_zero():
     assert ref.off(layer_norm(x), *ref.norm(x.double(), None, None, 1e-5)["h"]) <= 1
 
 
+@pytest.mark.parametrize("d,value,dtype", [(5, 2.0 ** 123, F32), (65, 2.0 ** 120, F32), (9, 2.0 ** 122, BF16), (300, 2.0 ** 118, F32)])
+def test_layer_norm_gradient_of_huge_equal_values(d, value, dtype):
+    """Equal values near float32's end: the differences are 0, though the mean times 1 / sqrt(eps) has no float32."""
+    from master_doko_reinforcement_learning_amd import layer_norm
+    eps = 1e-5 if d < 300 else 1e-8
+    x = torch.full((3, d), value, device=DEV, dtype=dtype, requires_grad=True)
+    w = torch.ones(d, device=DEV, dtype=dtype, requires_grad=True)
+    dh = _randn(_gen(d), 3, d, dtype=dtype)
+    h = layer_norm(x, w, eps=eps)
+    assert not h.any()
+    dx, dw = torch.autograd.grad(h, (x, w), dh)
+    g = dh.double()
+    want = (g - g.mean(-1, keepdim=True)) / math.sqrt(eps)
+    # (the mean: d / 64 + 16 additions; the root, its quotient, eps and the products: 8 more steps)
+    tol = ref.half_step(want, dtype) + ref.U * (d / 64 + 24) * (g.abs() + g.abs().mean(-1, keepdim=True)) / math.sqrt(eps)
+    assert ref.off(dx, want, tol) <= 1 and not dw.any()
+
+
 def test_layer_norm_equal_bits():
     from master_doko_reinforcement_learning_amd import layer_norm
     x, delta, w, b, dh, dres = _norm_case(3001, 256, F32, F32, 10, True)
@@ -716,6 +734,40 @@ def test_adamw_state_dict_round_trip():
     mine.step()
     assert int(mine.state[twin[0]]["step"]) == 2
     torch.testing.assert_close(twin[0], plain[0], rtol=2e-6, atol=2e-8)   # two f32 forms of one formula: ~30 u of p, of a step
+
+
+def test_adamw_refuses_shared_memory():
+    """A parameter given twice, or two that overlap, would be updated by two workgroups at once."""
+    from master_doko_reinforcement_learning_amd import AdamW
+    flat = torch.zeros(1000, device=DEV)
+    a, b, c = (flat[lo:lo + 300].detach().requires_grad_() for lo in (0, 300, 599))
+    AdamW([b, a])
+    with pytest.raises(ValueError, match="overlap"):
+        AdamW([a, b, c])
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="overlap"):
+        AdamW([a, a])
+
+
+def test_adamw_load_keeps_the_device_lr():
+    """A learning rate on the device stays the tensor that a captured step reads, and takes the loaded value; what a
+    scheduler keeps in the groups is loaded too."""
+    from master_doko_reinforcement_learning_amd import AdamW
+    p, q = (torch.ones(5, device=DEV, requires_grad=True) for _ in range(2))
+    lr = torch.tensor([0.5], device=DEV)
+    mine, theirs = AdamW([p], lr=lr), AdamW([q], lr=torch.tensor(0.25, device=DEV))
+    torch.optim.lr_scheduler.StepLR(theirs, 1)
+    mine.load_state_dict(theirs.state_dict())
+    assert mine.param_groups[0]["lr"] is lr and lr.item() == 0.25 and "initial_lr" in mine.param_groups[0]
+    theirs.param_groups[0]["lr"].fill_(1.0)
+    assert lr.item() == 0.25
+    mine.load_state_dict(AdamW([q], lr=0.125).state_dict())
+    assert lr.item() == 0.125
+    plain = AdamW([p], lr=0.5)
+    plain.load_state_dict(theirs.state_dict())
+    theirs.param_groups[0]["lr"].fill_(2.0)
+    assert float(plain.param_groups[0]["lr"]) == 1.0
+    with pytest.raises(ValueError, match="maximize"):
+        plain.load_state_dict(torch.optim.AdamW([q], maximize=True).state_dict())
 
 
 def test_adamw_copies():

@@ -55,13 +55,13 @@ def test_token_logprobs_entries_refuse():
     def forward(x=p, rows=1, vocab=8, type=0, temperature=1.0, tokens=p, n=1, top=0, lp=p, tl=None, tt=None):
         return L.dk_net_token_logprobs_async(x, vocab, rows, vocab, type, None, 0, temperature, tokens, n, top, lp, None, None, tl, tt, None, 0, None)
     for bad in (dict(type=4), dict(vocab=0), dict(n=65), dict(top=33), dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=float("inf")),
-                dict(x=None), dict(tokens=None), dict(lp=None), dict(top=1), dict(top=1, tl=p), dict(rows=1 << 33)):
+                dict(temperature=1e-40), dict(temperature=2e30), dict(x=None), dict(tokens=None), dict(lp=None), dict(top=1), dict(top=1, tl=p), dict(rows=1 << 33)):
         assert forward(**bad) == INVALID, bad
     assert forward(rows=0, x=None) == 0
 
     def backward(x=p, rows=1, vocab=8, type=0, temperature=1.0, tokens=p, n=1, lp=p, lse=p, ent=p, dx=p):
         return L.dk_net_token_logprobs_bwd_async(x, vocab, rows, vocab, type, None, 0, temperature, tokens, n, lp, lse, ent, None, None, dx, None)
-    for bad in (dict(type=4), dict(vocab=0), dict(n=65), dict(temperature=-1.0), dict(x=None), dict(tokens=None), dict(lp=None), dict(lse=None), dict(ent=None), dict(dx=None)):
+    for bad in (dict(type=4), dict(vocab=0), dict(n=65), dict(temperature=-1.0), dict(temperature=1e-40), dict(x=None), dict(tokens=None), dict(lp=None), dict(lse=None), dict(ent=None), dict(dx=None)):
         assert backward(**bad) == INVALID, bad
     assert backward(rows=0, x=None) == 0
 
