@@ -486,7 +486,9 @@ __device__ __forceinline__ float token_gradient(const LogpBwdArgs& a, uint64_t r
 struct RowGrad {
     float inv_t, m, log_s, total, ge, ent;
     __device__ float of(float v) const {
-        const float lp = (v - m) * inv_t - log_s, d = -raw_exp2(lp * LOG2E) * (total + ge * (lp + ent));
+        const float lp = (v - m) * inv_t - log_s, p = raw_exp2(lp * LOG2E);
+        // (p log p is 0 where p is: log p may have left f32 there, as with logits of the type's lowest value)
+        const float d = -p * (total + ge * (p == 0.0f ? 0.0f : lp + ent));
         return v == NEG_INF ? 0.0f : d;
     }
 };
