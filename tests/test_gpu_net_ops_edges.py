@@ -68,3 +68,25 @@ def test_gradient_of_the_types_lowest_values(vocab, dtype, temperature):
     leaf = x.detach().requires_grad_()
     dx, = torch.autograd.grad(token_logprobs(leaf, t, temperature=temperature).logprobs, leaf, bad)
     assert not dx[2].isfinite().all() and dx[[0, 1, 3, 4, 5]].isfinite().all()
+
+
+@pytest.mark.parametrize("vocab", [39, 700, 9001])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_disallowed_entries_of_nan_rows_take_no_gradient(vocab, dtype):
+    """A NaN or +inf in an allowed entry makes its row NaN; masked entries and those of -inf still take nothing, also where
+    they are among the row's tokens."""
+    from master_doko_reinforcement_learning_amd import token_logprobs
+    g = _gen(vocab)
+    x = _randn(g, 4, vocab, dtype=dtype)
+    mask = torch.rand(4, vocab, generator=g, device=DEV) < 0.5
+    mask[:, 0], mask[:, 1], mask[:, 2], mask[:, 3] = True, False, True, False
+    x[0, 0], x[1, 0], x[2, 0] = math.nan, math.inf, -math.inf
+    x[:, 2] = -math.inf
+    x[:, 3] = math.nan
+    t = torch.tensor([[1, 2, 4, 1]] * 4, device=DEV)
+    leaf = x.requires_grad_()
+    got = token_logprobs(leaf, t, mask=mask)
+    dx, = torch.autograd.grad([got.logprobs, got.entropy], [leaf], [_randn(g, 4, 4), _randn(g, 4)])
+    dead = ~mask | (x.detach() == -math.inf)
+    assert not dx[dead].any()
+    assert dx[:2][~dead[:2]].isnan().all() and dx[2:].isfinite().all()
