@@ -18,7 +18,7 @@ import torch
 from . import _native
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # enum dk_net_type
-NORM_MAX_D, TOKENS_MAX, TOP_MAX, ADAMW_BLOCK = 16384, 64, 32, 256
+NORM_MAX_D, VOCAB_MAX, TOKENS_MAX, TOP_MAX, ADAMW_BLOCK = 16384, (1 << 31) - 1, 64, 32, 256
 
 
 def _check(rc, what):
@@ -225,8 +225,8 @@ def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
     logit holds is not looked at (nor has one a gradient whose log probability is below float32's range).  A row with nothing allowed has entropy 0.  Alternatives are ordered by
     logit, equal ones by index; -1 (and -inf) behind the last allowed one."""
     _floating(logits, "token_logprobs")
-    if logits.dim() == 0 or logits.shape[-1] == 0:
-        raise ValueError("token_logprobs: logits need a last dimension of at least 1, got %s" % (tuple(logits.shape),))
+    if logits.dim() == 0 or not 0 < logits.shape[-1] <= VOCAB_MAX:   # (the entries take 32 bits of it)
+        raise ValueError("token_logprobs: a vocabulary of 1 to %d, got logits %s" % (VOCAB_MAX, tuple(logits.shape)))
     lead = logits.shape[:-1]
     if tokens is not None:
         if tokens.device != logits.device or tokens.dtype not in (torch.int64, torch.int32):

@@ -90,3 +90,11 @@ def test_disallowed_entries_of_nan_rows_take_no_gradient(vocab, dtype):
     dead = ~mask | (x.detach() == -math.inf)
     assert not dx[dead].any()
     assert dx[:2][~dead[:2]].isnan().all() and dx[2:].isfinite().all()
+
+
+def test_vocabularies_past_32_bits_are_refused():
+    from master_doko_reinforcement_learning_amd import token_logprobs
+    one = torch.zeros(1, dtype=BF16, device=DEV)
+    for vocab in (1 << 31, (1 << 32) + 5):
+        with pytest.raises(ValueError):
+            token_logprobs(one.expand(vocab))
