@@ -3,7 +3,7 @@ probabilities of given tokens with entropy and top alternatives, and AdamW over 
 
 Each is a HIP kernel behind the C-ABI (dk_net_layer_norm_*, dk_net_token_logprobs_*,
 dk_net_adamw_async; csrc/train_*_kernels.h) on torch's current stream of the tensors' device, and the
-first two are differentiable (once).  f32, bf16 and f16; sums and statistics are f32.  There is no CPU
+first two are differentiable (once, in reverse mode).  f32, bf16 and f16; sums and statistics are f32.  There is no CPU
 fallback.  DokoAzNet.loss / DokoImpiNet.loss are built on the first two, NetTrainer on all three.
 """
 import collections
@@ -14,6 +14,7 @@ from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -55,6 +56,12 @@ def _floating(t, what):
     if t.dtype not in _TYPES:
         raise ValueError("%s: float32, bfloat16 or float16 is needed, got %s" % (what, t.dtype))
     return _TYPES[t.dtype]
+
+
+def _no_tangents(what, *tensors):
+    """Raises for a forward-mode dual tensor: the kernels would read its values and drop its tangent."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("%s has no forward-mode derivative" % what)
 
 
 def _ptr(t):
@@ -143,6 +150,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, delta=None):
             raise ValueError("layer_norm: weight and bias are [%d] tensors in %s or float32 on %s" % (x.shape[-1], x.dtype, x.device))
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("layer_norm: weight and bias differ in dtype")
+    _no_tangents("layer_norm", x, delta, weight, bias)
     weight = weight if weight is None else weight.contiguous()
     bias = bias if bias is None else bias.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, weight, bias)):
@@ -242,6 +250,7 @@ def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
         raise ValueError("token_logprobs: temperature %r (1e-6 to 1e30)" % (temperature,))
     if not 0 <= top <= TOP_MAX:
         raise ValueError("token_logprobs: top %r (0 to %d)" % (top, TOP_MAX))
+    _no_tangents("token_logprobs", logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, mask, temperature, top))
     logprobs, entropy, _, tl, tt, _ = _logp_forward(logits, tokens, mask, temperature, top, False)
