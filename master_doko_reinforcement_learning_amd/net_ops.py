@@ -141,12 +141,12 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, delta=None):
         raise ValueError("layer_norm: 1 to %d columns, got %s" % (NORM_MAX_D, tuple(x.shape)))
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError("layer_norm: eps %r" % (eps,))
-    if delta is not None and (delta.shape != x.shape or delta.dtype != x.dtype or delta.device != x.device):
+    if delta is not None and (not isinstance(delta, torch.Tensor) or delta.shape != x.shape or delta.dtype != x.dtype or delta.device != x.device):
         raise ValueError("layer_norm: delta has x's shape, dtype and device")
     for t in (weight, bias):
         if t is None:
             continue
-        if t.device != x.device or t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32):
+        if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32):
             raise ValueError("layer_norm: weight and bias are [%d] tensors in %s or float32 on %s" % (x.shape[-1], x.dtype, x.device))
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("layer_norm: weight and bias differ in dtype")
@@ -237,13 +237,14 @@ def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
         raise ValueError("token_logprobs: a vocabulary of 1 to %d, got logits %s" % (VOCAB_MAX, tuple(logits.shape)))
     lead = logits.shape[:-1]
     if tokens is not None:
-        if tokens.device != logits.device or tokens.dtype not in (torch.int64, torch.int32):
+        if not isinstance(tokens, torch.Tensor) or tokens.device != logits.device or tokens.dtype not in (torch.int64, torch.int32):
             raise ValueError("token_logprobs: tokens are int64 or int32 on the logits' device")
         if tokens.shape != lead and not (tokens.dim() == len(lead) + 1 and tokens.shape[:-1] == lead and tokens.shape[-1] <= TOKENS_MAX):
             raise ValueError("token_logprobs: tokens %s do not go with logits %s (at most %d a row)"
                              % (tuple(tokens.shape), tuple(logits.shape), TOKENS_MAX))
         tokens = tokens.long().contiguous()
-    if mask is not None and (mask.device != logits.device or mask.dtype != torch.bool or mask.shape not in (logits.shape, logits.shape[-1:])):
+    if mask is not None and (not isinstance(mask, torch.Tensor) or mask.device != logits.device or mask.dtype != torch.bool
+                             or mask.shape not in (logits.shape, logits.shape[-1:])):
         raise ValueError("token_logprobs: mask is bool on the logits' device, in their shape or [%d]" % logits.shape[-1])
     temperature = float(temperature)
     if not 1e-6 <= temperature <= 1e30:

@@ -117,3 +117,12 @@ def test_forward_mode_tangents_are_refused():
         assert torch.equal(layer_norm(x, w), layer_norm(forward_ad.unpack_dual(d).primal, w))   # without a tangent as ever
         token_logprobs(grad, t).logprobs.sum().backward()
     assert torch.equal(layer_norm(d, dw), layer_norm(x, w))   # (the level is over, and the tangents with it)
+
+
+def test_arguments_that_are_no_tensors_are_refused():
+    from master_doko_reinforcement_learning_amd import layer_norm, token_logprobs
+    x = torch.zeros(2, 8, device=DEV)
+    for bad in (lambda: layer_norm(x, [1.0] * 8), lambda: layer_norm(x, None, 0.0), lambda: layer_norm(x, delta=[x]), lambda: token_logprobs(x, [0, 0]),
+                lambda: token_logprobs(x, 0), lambda: token_logprobs(x, mask=[True] * 8)):
+        with pytest.raises(ValueError):
+            bad()
