@@ -260,7 +260,8 @@ def token_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0):
 
 # ------------------------------------------------------------------------------- AdamW
 _GRAD, _DTYPE = operator.attrgetter("grad"), operator.attrgetter("dtype")
-_DENSE, _PTR, _INDEX = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.get_device   # (-1 on the CPU)
+_DENSE, _NUMEL, _PTR = torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.data_ptr
+_INDEX = torch.Tensor.get_device   # (-1 on the CPU)
 _ROW = np.dtype([("p", np.uint64), ("g", np.uint64), ("n", np.uint64), ("block", np.uint64), ("id", np.uint64)])
 
 
@@ -348,7 +349,7 @@ class AdamW(torch.optim.Optimizer):
                 st["master"].copy_(p)
         # (scratch of a step: the tensors' factors; and the parameters' versions that the masters go with)
         self.buffers.append(b)
-        self._tables.append({"rows": table, "dtype": params[0].dtype if params else None, "device": dev,
+        self._tables.append({"rows": table, "sizes": [p.numel() for p in params], "dtype": params[0].dtype if params else None, "device": dev,
                              "factors": torch.empty(3 * max(1, len(params)), dtype=torch.float32, device=dev),
                              "versions": [p._version for p in params] if master else None})
 
@@ -367,23 +368,24 @@ class AdamW(torch.optim.Optimizer):
         lr, d_lr = _hyper(group)
         if d_lr is not None and d_lr.device != device:
             raise ValueError("AdamW: lr lies on another device than its group")
-        params, at = group["params"], None
+        params, sizes, at = group["params"], t["sizes"], None
         grads = list(map(_GRAD, params))
         if not all(map(operator.is_not, grads, itertools.repeat(None))):
             at = [i for i, g in enumerate(grads) if g is not None]
-            params, grads = [params[i] for i in at], [grads[i] for i in at]
+            params, grads, sizes = [params[i] for i in at], [grads[i] for i in at], [sizes[i] for i in at]
             if not params:
                 return
         # (checked anew each step, in maps: a network has a hundred tensors, and the step takes 20 us on the GPU)
-        if set(map(_DTYPE, params)) != {dtype} or set(map(_INDEX, params)) != {device.index} or not all(map(_DENSE, params)):
-            raise RuntimeError("AdamW: a parameter was moved, cast or restrided since the optimiser was made")
+        if (list(map(_NUMEL, params)) != sizes or set(map(_DTYPE, params)) != {dtype} or set(map(_INDEX, params)) != {device.index}
+                or not all(map(_DENSE, params))):
+            raise RuntimeError("AdamW: a parameter was moved, cast, resized or restrided since the optimiser was made")
         try:
-            if set(map(_DTYPE, grads)) != {dtype}:
+            if set(map(_DTYPE, grads)) != {dtype} or list(map(_NUMEL, grads)) != sizes:
                 raise RuntimeError
             if not all(map(_DENSE, grads)):   # (raises for a sparse one)
                 grads = [g.contiguous() for g in grads]
         except RuntimeError:
-            raise ValueError("AdamW: gradients are dense and in the parameters' dtype") from None
+            raise ValueError("AdamW: gradients are dense and of the parameters' sizes and dtype") from None
         versions = t["versions"]
         if versions is not None:
             for i, p in zip(at or range(len(params)), params):
