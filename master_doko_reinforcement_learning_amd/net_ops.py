@@ -318,15 +318,14 @@ class AdamW(torch.optim.Optimizer):
             _floating(p, "AdamW")
             if p.dtype != params[0].dtype or p.device != params[0].device or not p.is_contiguous():
                 raise ValueError("AdamW: a group's parameters are dense and share one dtype and device")
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):   # (they are updated side by side)
+        if _overlap(params):
             raise ValueError("AdamW: a group's parameters overlap, or one is given twice")
         master = self.master_weights and bool(params) and params[0].dtype != torch.float32
         dev = params[0].device if params else None
         table = np.zeros(len(params), _ROW)
         blocks = 0
         for i, p in enumerate(params):
-            table[i] = (0, 0, p.numel(), blocks, i)
+            table[i] = (p.data_ptr(), 0, p.numel(), blocks, i)
             blocks += -(-p.numel() // ADAMW_BLOCK)
         b = {"step": torch.zeros(len(params), dtype=torch.int32, device=dev)}
         for k in ("exp_avg", "exp_avg_sq"):
@@ -393,7 +392,11 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p]["master"].copy_(p)
         n = len(params)
         rows = t["rows"] if at is None else t["rows"][at]
-        rows["p"] = np.fromiter(map(_PTR, params), np.uint64, n)
+        memory = np.fromiter(map(_PTR, params), np.uint64, n)
+        if not np.array_equal(memory, rows["p"]):   # (new memory, through p.data: looked at as the first was)
+            if _overlap(group["params"]):
+                raise RuntimeError("AdamW: a group's parameters overlap since the optimiser was made")
+            t["rows"]["p"][slice(None) if at is None else at] = rows["p"] = memory
         rows["g"] = np.fromiter(map(_PTR, grads), np.uint64, n)
         b1, b2 = group["betas"]
         _check(_launch(_native.lib().dk_net_adamw_async, device.index, rows.ctypes.data, n, _TYPES[dtype], self.state_bits,
@@ -442,6 +445,12 @@ class AdamW(torch.optim.Optimizer):
         for t, g in zip(self._tables, self.param_groups):
             if t["versions"] is not None:
                 t["versions"] = [p._version for p in g["params"]]
+
+
+def _overlap(params):
+    """Whether two parameters share memory: a group's are updated side by side."""
+    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
 
 
 def _hyper(group):

@@ -53,3 +53,22 @@ def test_adamw_refuses_another_number_of_elements(adamw):
         ps[0].grad = torch.ones(300)
         opt.step()
         assert [t[2] for t in launches.pop()] == [300, 7]
+
+
+def test_adamw_refuses_memory_that_came_to_be_shared(adamw):
+    """Two parameters of a group on the same memory since the optimiser was made: two workgroups would update it at once."""
+    AdamW, launches = adamw
+    for shared in (lambda a: a.data, lambda a: a.data[100:].view(-1)):
+        a, b, c = _params(300, 200, 9)
+        opt = AdamW([a, b, c])
+        opt.step()
+        b.data = shared(a)[:200]
+        for grad in (torch.ones(300), None, torch.ones(300)):
+            a.grad = grad
+            launches.clear()
+            with pytest.raises(RuntimeError, match="overlap"):
+                opt.step()
+            assert not launches
+        b.data = torch.zeros(200)
+        opt.step()
+        assert [(t[0], t[2]) for t in launches.pop()] == [(p.data_ptr(), p.numel()) for p in (a, b, c)]
