@@ -1,5 +1,6 @@
 """The training operators (net_ops.py) on the GPU where their formulas leave float32's range, where a caller writes to
 what an optimiser keeps a copy of, and where a call has to be refused."""
+import copy
 import math
 
 import pytest
@@ -126,3 +127,17 @@ def test_arguments_that_are_no_tensors_are_refused():
                 lambda: token_logprobs(x, 0), lambda: token_logprobs(x, mask=[True] * 8)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_adamw_empty_groups():
+    """A group without parameters does nothing, also under a learning rate on the device."""
+    from master_doko_reinforcement_learning_amd import AdamW
+    lr = torch.tensor(0.5, device=DEV)
+    for bits, dtype in ((32, F32), (8, BF16)):
+        p = torch.zeros(3, device=DEV, dtype=dtype, requires_grad=True)
+        p.grad = torch.ones_like(p)
+        opt = AdamW([{"params": []}, {"params": [p]}], lr=lr, weight_decay=0.0, state_bits=bits, master_weights=True)
+        opt.step()
+        assert (p == -0.5).all()
+        opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+        copy.deepcopy(opt).step()

@@ -72,3 +72,11 @@ def test_adamw_refuses_memory_that_came_to_be_shared(adamw):
         b.data = torch.zeros(200)
         opt.step()
         assert [(t[0], t[2]) for t in launches.pop()] == [(p.data_ptr(), p.numel()) for p in (a, b, c)]
+
+
+def test_adamw_steps_with_an_empty_group(adamw):
+    AdamW, launches = adamw
+    p, = _params(5)
+    opt = AdamW([{"params": []}, {"params": [p]}])
+    opt.step()
+    assert [t[2] for t in launches.pop()] == [5]
