@@ -412,7 +412,11 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes over the states of a state_dict() of the same parameters, into the buffers that are there
-        (also torch.optim.AdamW's, where state_bits is 32)."""
+        (also torch.optim.AdamW's, where state_bits is 32); runs the hooks registered for it."""
+        state_dict = dict(state_dict)   # (a hook may write to it)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the state_dict has other parameter groups")
@@ -445,6 +449,8 @@ class AdamW(torch.optim.Optimizer):
         for t, g in zip(self._tables, self.param_groups):
             if t["versions"] is not None:
                 t["versions"] = [p._version for p in g["params"]]
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
 
 def _overlap(params):

@@ -80,3 +80,30 @@ def test_adamw_steps_with_an_empty_group(adamw):
     opt = AdamW([{"params": []}, {"params": [p]}])
     opt.step()
     assert [t[2] for t in launches.pop()] == [5]
+
+
+def test_adamw_load_state_dict_hooks(adamw):
+    """Registered hooks run: one before, which may replace the state_dict, and one after it is loaded."""
+    AdamW, _ = adamw
+    ps, qs = _params(300, 7), _params(300, 7)
+    opt, other = AdamW(ps, lr=0.25), AdamW(qs)
+    opt.state[ps[0]]["exp_avg"].fill_(2.0)
+    seen = []
+
+    def before(o, state_dict):
+        seen.append(("before", o, float(o.state[qs[0]]["exp_avg"][0])))
+        state_dict["param_groups"] = [dict(g, lr=0.5) for g in state_dict["param_groups"]]   # (of its own copy)
+
+    def replaced(o, state_dict):
+        seen.append(("replaced", o, state_dict["param_groups"][0]["lr"]))
+        return dict(state_dict, param_groups=[dict(g, eps=0.125) for g in state_dict["param_groups"]])
+    other.register_load_state_dict_pre_hook(before)
+    handle = other.register_load_state_dict_pre_hook(replaced)
+    other.register_load_state_dict_post_hook(lambda o: seen.append(("after", o, float(o.state[qs[0]]["exp_avg"][0]))))
+    state = opt.state_dict()
+    other.load_state_dict(state)
+    assert seen == [("before", other, 0.0), ("replaced", other, 0.5), ("after", other, 2.0)]
+    assert other.param_groups[0]["lr"] == 0.5 and other.param_groups[0]["eps"] == 0.125 and state["param_groups"][0]["lr"] == 0.25
+    handle.remove()
+    other.load_state_dict(state)
+    assert other.param_groups[0]["eps"] == 1e-8
