@@ -271,7 +271,9 @@ class AdamW(torch.optim.Optimizer):
     state_bits 32: f32 moments.  state_bits 8: e4m3 codes of exp_avg and of sqrt(exp_avg_sq) with one f32
     scale for each 256 elements of a tensor.  master_weights: bf16 / f16 parameters are rounded copies of
     f32 weights that the optimiser keeps; a parameter that was written to since the last step (a loaded
-    state_dict) is taken over into its master first.  lr may be a one-element f32 tensor on the GPU.
+    state_dict) is taken over into its master first.  step() sees that by the parameter's version counter, which
+    a write through .data does not raise, and a captured step does not look: refresh_masters() takes over what was
+    written in such ways, and before a capture.  lr may be a one-element f32 tensor on the GPU.
 
     A group's parameters share one dtype and device, are dense and do not overlap.  The states lie in flat buffers
     (`buffers`, one dict a group; each parameter at a multiple of 256 elements) and state[p] holds views of
@@ -387,9 +389,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: gradients are dense and of the parameters' sizes and dtype") from None
         versions = t["versions"]
         if versions is not None:
-            for i, p in zip(at or range(len(params)), params):
-                if versions[i] != p._version:
-                    self.state[p]["master"].copy_(p)
+            self._take_over(t, [(i, p) for i, p in zip(at or range(len(params)), params) if versions[i] != p._version])
         n = len(params)
         rows = t["rows"] if at is None else t["rows"][at]
         memory = np.fromiter(map(_PTR, params), np.uint64, n)
@@ -408,6 +408,29 @@ class AdamW(torch.optim.Optimizer):
         if versions is not None:
             for i, p in zip(at or range(n), params):
                 versions[i] = p._version
+
+    @torch.no_grad()
+    def refresh_masters(self):
+        """Takes every parameter whose values are not its rounded master's over into the master: written to through
+        .data, between the replays of a captured step, or before one is captured (not within a capture itself)."""
+        for group, t in zip(self.param_groups, self._tables):
+            if t["versions"] is not None:
+                self._take_over(t, list(enumerate(group["params"])))
+
+    def _take_over(self, t, written):
+        """The masters of the parameters `written`, (place in the group, parameter) each.  One whose values are its rounded
+        master's keeps that, which holds more of them: its version counter may be raised by others than writers."""
+        if not written:
+            return
+        with torch.cuda.device(t["device"]):
+            if torch.cuda.is_current_stream_capturing():   # (each replay would round the masters)
+                raise RuntimeError("AdamW: a parameter was written to since the last step: refresh_masters() before the capture")
+        for i, p in written:
+            master, values = self.state[p]["master"].view(-1), p.detach().reshape(-1).to(t["device"])
+            if values.numel() != master.numel():
+                raise RuntimeError("AdamW: a parameter was resized since the optimiser was made")
+            torch.where((master.to(t["dtype"]) == values).all(), master, values, out=master)
+            t["versions"][i] = p._version
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):

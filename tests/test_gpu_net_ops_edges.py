@@ -141,3 +141,80 @@ def test_adamw_empty_groups():
         assert (p == -0.5).all()
         opt.load_state_dict(copy.deepcopy(opt.state_dict()))
         copy.deepcopy(opt).step()
+
+
+# ------------------------------------------------------------------------------------ AdamW's masters
+def _with_masters(seed, **kw):
+    from master_doko_reinforcement_learning_amd import AdamW
+    g = _gen(seed)
+    params = [_randn(g, n, dtype=BF16, scale=0.5).requires_grad_() for n in (300, 5, 1024)]
+    for p in params:
+        p.grad = _randn(g, *p.shape, dtype=BF16)
+    return params, AdamW(params, lr=1e-5, weight_decay=0.0, master_weights=True, **kw)   # (far below half a step of most weights)
+
+
+def _same(a, b):
+    (ps, o), (qs, u) = a, b
+    return all(torch.equal(p, q) and torch.equal(o.state[p]["master"], u.state[q]["master"]) and torch.equal(p, o.state[p]["master"].to(p.dtype))
+               for p, q in zip(ps, qs))
+
+
+def _write(params, value):
+    with torch.no_grad():
+        for i, p in enumerate(params):
+            p.copy_(torch.linspace(-value, value + i, p.numel(), device=DEV))
+
+
+def test_captured_step_keeps_the_masters():
+    """A step whose parameters were written to is not captured: each replay would take the rounded weights over.  After
+    refresh_masters it is, and its replays are the eager steps."""
+    want, mine = _with_masters(1), _with_masters(1)
+    for params, opt in (want, mine):
+        opt.step()
+        _write(params, 0.7)                    # the weights of before a warm-up, say
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        two = torch.ones(1, device=DEV) + 1
+        with pytest.raises(RuntimeError, match="refresh_masters"):
+            mine[1].step()
+    graph.replay()
+    assert float(two) == 2
+    mine[1].refresh_masters()
+    assert all(torch.equal(mine[1].state[p]["master"], p.float()) and int(mine[1].state[p]["step"]) == 1 for p in mine[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mine[1].step()
+    for _ in range(4):
+        graph.replay()
+        want[1].step()
+        torch.cuda.synchronize()
+        assert _same(want, mine)
+    assert any((mine[1].state[p]["master"] != p.float()).any() for p in mine[0])
+    # what is written between replays is taken over where the caller says so
+    for params, _ in (want, mine):
+        _write(params, 0.3)
+    mine[1].refresh_masters()
+    for _ in range(3):
+        graph.replay()
+        want[1].step()
+        torch.cuda.synchronize()
+        assert _same(want, mine)
+
+
+def test_raised_version_counters_leave_the_masters():
+    """A parameter that holds its rounded master was not written to, whatever its version counter says (a caller raises it
+    after a replay, for the networks' fused forwards)."""
+    want, mine = _with_masters(2), _with_masters(2)
+    for _ in range(4):
+        want[1].step()
+        mine[1].step()
+        torch.autograd.graph.increment_version(mine[0])
+        assert _same(want, mine)
+    mine[1].refresh_masters()
+    assert _same(want, mine)
+    # a write through .data raises no counter: refresh_masters finds it
+    for params, opt in (want, mine):
+        for p in params:
+            p.data.copy_(torch.linspace(-0.2, 0.9, p.numel(), device=DEV))
+        opt.refresh_masters()
+        assert all(torch.equal(opt.state[p]["master"], p.float()) for p in params)
