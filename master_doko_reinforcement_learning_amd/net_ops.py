@@ -288,7 +288,9 @@ class AdamW(torch.optim.Optimizer):
         self.buffers, self._tables = [], []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    @torch.no_grad()
     def __getstate__(self):   # (a copy or a pickle, which knows no e4m3: the codes as bytes; the buffers are laid out anew)
+        self._take_over_written()
         state = super().__getstate__()
         state["state"] = {p: {k: v.view(torch.uint8) if v.dtype == torch.float8_e4m3fn else v for k, v in st.items()}
                           for p, st in state["state"].items()}
@@ -416,6 +418,17 @@ class AdamW(torch.optim.Optimizer):
         for group, t in zip(self.param_groups, self._tables):
             if t["versions"] is not None:
                 self._take_over(t, list(enumerate(group["params"])))
+
+    def _take_over_written(self):   # (what step() would see)
+        for group, t in zip(self.param_groups, self._tables):
+            if t["versions"] is not None:
+                self._take_over(t, [(i, p) for i, p in enumerate(group["params"]) if t["versions"][i] != p._version])
+
+    @torch.no_grad()
+    def state_dict(self):
+        """torch.optim.Optimizer.state_dict; the masters in it go with the parameters as they are."""
+        self._take_over_written()
+        return super().state_dict()
 
     def _take_over(self, t, written):
         """The masters of the parameters `written`, (place in the group, parameter) each.  One whose values are its rounded

@@ -218,3 +218,25 @@ def test_raised_version_counters_leave_the_masters():
             p.data.copy_(torch.linspace(-0.2, 0.9, p.numel(), device=DEV))
         opt.refresh_masters()
         assert all(torch.equal(opt.state[p]["master"], p.float()) for p in params)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_follow_written_parameters(bits):
+    """Parameters that were written to after the last step: a copy, a state_dict and the optimiser itself go on from the
+    written values."""
+    from master_doko_reinforcement_learning_amd import AdamW
+    params, opt = _with_masters(3, state_bits=bits)
+    opt.step()
+    _write(params, 0.4)
+    qs, twin = copy.deepcopy((params, opt))
+    rs = [p.detach().clone().requires_grad_() for p in params]
+    other = AdamW(rs, lr=1.0, weight_decay=0.0, master_weights=True, state_bits=bits)
+    other.load_state_dict(opt.state_dict())
+    for p, q, r in zip(params, qs, rs):
+        q.grad, r.grad = p.grad.clone(), p.grad.clone()
+    for _ in range(2):
+        opt.step()
+        twin.step()
+        other.step()
+        assert _same((params, opt), (qs, twin)) and _same((params, opt), (rs, other))
+    assert all((opt.state[p]["master"].abs() < 3).all() and (p[-1] > 0.3) for p in params)
