@@ -635,8 +635,8 @@ enum dk_net_type { DK_F32 = 0, DK_BF16 = 1, DK_F16 = 2 };
 /* dk_net_layer_norm_async: x_out = x + delta (rounded to `type`), h_out = LayerNorm(x_out; gamma, beta,
  * eps) over d <= 16384 columns; delta NULL: h_out = LayerNorm(x), x_out may be NULL.  gamma / beta are of
  * `wtype` (DK_F32 or `type`), NULL for 1 / 0.  stats [rows][2] (or NULL) receives each row's mean and
- * 1 / sqrt(var + eps) for the backward pass.  x_out and h_out are dense [rows][d]; x_out may be x, or delta
- * where that is dense.
+ * 1 / sqrt(var + eps) for the backward pass.  x_out and h_out are dense [rows][d]; x_out may be x or
+ * delta where that one's rows are dense too (DK_E_INVALID where they are not).
  * dk_net_layer_norm_bwd_async: dh = the gradient of h_out, dx_res (or NULL) that of x_out, x the rows that
  * were normalised; dx [rows][d] is the gradient of x (and of delta), dgamma / dbeta [d] (either may be
  * NULL) are of `wtype`.  Without dgamma and dbeta the workspace may be NULL; otherwise it has

@@ -141,6 +141,8 @@ int dk_net_layer_norm_async(const void* x, uint64_t x_stride, const void* delta,
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
     if (!x || !h_out) return DK_E_INVALID;
+    // (x_out over rows of another pitch would overwrite some before they are read)
+    if (x_out && rows > 1 && ((x_out == x && x_stride != d) || (x_out == delta && delta_stride != d))) return DK_E_INVALID;
     const NormArgs a{x, delta, x_stride, delta_stride, rows, d, wtype == DK_F32, gamma, beta, eps, 1.0f / (float)d, x_out, h_out, stats};
     with_type(type, [&](auto t) {
         using T = decltype(t);

@@ -1,10 +1,13 @@
 """Refusals and bookkeeping of the training operators (net_ops.py) without a GPU: the optimiser on CPU tensors with its
 launches recorded in place of run, and the C entries' answers to arguments that no launch may see."""
+import ctypes
 
 import pytest
 import torch
 
 from master_doko_reinforcement_learning_amd import _native
+
+INVALID = -1
 
 
 @pytest.fixture
@@ -107,3 +110,15 @@ def test_adamw_load_state_dict_hooks(adamw):
     handle.remove()
     other.load_state_dict(state)
     assert other.param_groups[0]["eps"] == 1e-8
+
+
+def test_layer_norm_entry_refuses_strided_rows_in_place():
+    """x_out is dense: over x or delta themselves only where their rows are."""
+    L = _native.lib()
+    buf, other = ctypes.create_string_buffer(4096), ctypes.create_string_buffer(4096)
+    p, q = ctypes.addressof(buf), ctypes.addressof(other)
+
+    def forward(x=p, x_stride=8, delta=q, delta_stride=8, x_out=p):
+        return L.dk_net_layer_norm_async(x, x_stride, delta, delta_stride, 2, 8, 0, None, None, 0, 1e-5, x_out, ctypes.addressof(other) + 1024, None, None)
+    assert forward(x_stride=9) == INVALID and forward(x_stride=0) == INVALID and forward(delta=None, x_stride=16) == INVALID
+    assert forward(x_out=q, delta_stride=12) == INVALID and forward(x_out=q, delta_stride=0) == INVALID
