@@ -50,7 +50,8 @@ class DokoImpiNet(nn.Module):
         """The differentiable forward on the GPU (f32): forward_torch with every residual add and LayerNorm of
         the blocks in one kernel, forward and backward."""
         x = embed_tokens(self.emb, tokens)
-        _, h = trunk_train(x, norm_train(x, self.blocks[0].ln_1), self.blocks, self.ln_f)
+        first = self.blocks[0].ln_1 if self.blocks else self.ln_f
+        _, h = trunk_train(x, norm_train(x, first), self.blocks, self.ln_f)
         return self.head(h, fused=False)
 
     def loss(self, tokens, guesses, mask=None):

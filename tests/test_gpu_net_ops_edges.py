@@ -240,3 +240,16 @@ def test_copies_follow_written_parameters(bits):
         other.step()
         assert _same((params, opt), (qs, twin)) and _same((params, opt), (rs, other))
     assert all((opt.state[p]["master"].abs() < 3).all() and (p[-1] > 0.3) for p in params)
+
+
+def test_impi_network_without_blocks():
+    """forward_train without blocks is the embedding, the last LayerNorm and the head, as forward_torch."""
+    from master_doko_reinforcement_learning_amd.impi_network import VOCAB_IPI, DokoImpiNet
+    torch.manual_seed(0)
+    net = DokoImpiNet(d=32, heads=4, layers=0).to(DEV)
+    tokens = torch.cat([torch.randint(0, v, (5, 62 if i < 5 else 1)) for i, v in enumerate(VOCAB_IPI)], dim=1).int().to(DEV)
+    got, want = net.forward_train(tokens), net.forward_torch(tokens)
+    # one LayerNorm of sums of 6 (32 columns) and a head's products of 32: ~100 roundings of values up to ~10 times the outputs' size
+    assert (got - want).abs().max() <= 100 * 10 * ref.U * want.abs().max().clamp(min=1)
+    net.loss(tokens, torch.arange(5, device=DEV)).backward()
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in net.parameters())
