@@ -93,6 +93,42 @@ def test_disallowed_entries_of_nan_rows_take_no_gradient(vocab, dtype):
     assert dx[:2][~dead[:2]].isnan().all() and dx[2:].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [39, 700, 3000, 9001, 40000])
+def test_results_do_not_depend_on_a_common_offset(vocab, dtype):
+    """Sums are of differences from the row's maximum: a common offset that leaves the logits exact leaves every bit, and a
+    row of the type's lowest value alone is the uniform distribution."""
+    from master_doko_reinforcement_learning_amd import token_logprobs
+    g = _gen(vocab)
+    # whole numbers of 0 to 15, f32: and 2^20, bf16: and 128 (8 bits hold 128 to 143)
+    x = torch.randint(0, 16, (5, vocab), generator=g, device=DEV).to(dtype)
+    t = torch.randint(0, vocab, (5, 3), generator=g, device=DEV)
+    dl, de = _randn(g, 5, 3), _randn(g, 5)
+    outs = []
+    for shift in (0.0, 2.0 ** 20 if dtype == F32 else 128.0, -2.0 ** 20 if dtype == F32 else -143.0):
+        z = x + shift
+        assert torch.equal(z.double() - shift, x.double())
+        leaf = z.requires_grad_()
+        got = token_logprobs(leaf, t, temperature=0.75, top=4)
+        dx, = torch.autograd.grad([got.logprobs, got.entropy], [leaf], [dl, de])
+        outs.append([o.detach() for o in got] + [dx])
+    for o in outs[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(o, outs[0]))
+    for temperature in (0.5, 1.0):
+        low = torch.full((2, vocab), torch.finfo(dtype).min, device=DEV, dtype=dtype, requires_grad=True)
+        got = token_logprobs(low, t[:2], temperature=temperature)
+        # log of a sum of `vocab` ones: whole numbers below 2^24 add up exactly, so one rounding of the logarithm (and 3 steps of it)
+        size = math.log(vocab)
+        assert (got.logprobs.detach().double() + size).abs().max() <= 4 * ref.U * size
+        assert (got.entropy.detach().double() - size).abs().max() <= 4 * ref.U * size
+        dx, = torch.autograd.grad(got.logprobs.sum(), low)
+        n = torch.zeros(2, vocab, device=DEV, dtype=torch.float64).scatter_add_(1, t[:2], torch.ones(2, 3, device=DEV, dtype=torch.float64))
+        want = (n - 3.0 / vocab) / temperature
+        # p = 2^(-log2 vocab): its argument is off by 4 u of it, so p by 4 u log2(vocab); the products and the sum by 8 u
+        tol = ref.half_step(want, dtype) + ref.U * (3.0 / vocab * (4 * math.log2(vocab) + 8) + 8 * n) / temperature
+        assert ref.off(dx, want, tol) <= 1
+
+
 def test_vocabularies_past_32_bits_are_refused():
     from master_doko_reinforcement_learning_amd import token_logprobs
     one = torch.zeros(1, dtype=BF16, device=DEV)
