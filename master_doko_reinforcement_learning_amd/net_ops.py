@@ -169,11 +169,16 @@ class TokenLogprobs(NamedTuple):
     top_tokens: Optional[torch.Tensor]
 
 
+def _mask_rows(mask):
+    """A mask as _rows has it; one of a single dimension goes for every row."""
+    return (None, 0) if mask is None else (mask.contiguous(), 0) if mask.dim() == 1 else _rows(mask)
+
+
 def _logp_forward(logits, tokens, mask, temperature, top, stats):
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     rows = logits.numel() // vocab
     xr, xs = _rows(logits)
-    mr, ms = (None, 0) if mask is None else (mask.contiguous(), 0) if mask.dim() == 1 and logits.dim() > 1 else _rows(mask)
+    mr, ms = _mask_rows(mask)
     n = 0 if tokens is None else 1 if tokens.dim() == len(lead) else tokens.shape[-1]
     f32 = torch.float32
     logprobs = None if tokens is None else logits.new_empty(tokens.shape, dtype=f32)
@@ -187,19 +192,20 @@ def _logp_forward(logits, tokens, mask, temperature, top, stats):
     _check(_launch(L.dk_net_token_logprobs_async, logits.get_device(), xr.data_ptr(), xs, rows, vocab, kind, _ptr(mr), ms, temperature,
                    _ptr(tokens), n, top, _ptr(logprobs), entropy.data_ptr(), _ptr(st), _ptr(tl), _ptr(tt), _ptr(ws), size),
            "token log probabilities")
-    return logprobs, entropy, st, tl, tt, (xr, mr, ms, n)
+    return logprobs, entropy, st, tl, tt, (xr, mr, n)
 
 
 def _logp_backward(ctx, dlogp, dent, _tl, _tt):
     if dlogp is None and dent is None:
         return None, None, None, None, None
     x, tokens, mask, logprobs, st, entropy = ctx.saved_tensors
-    xr, xs = _rows(x)
+    xr, xs = _rows(x)   # (saved tensors may come back with other strides: hooks copy them)
+    mr, ms = _mask_rows(mask)
     dlogp = None if dlogp is None else dlogp.contiguous()
     dent = None if dent is None else dent.contiguous()
     dx = x.new_empty(ctx.shape)
     _check(_launch(_native.lib().dk_net_token_logprobs_bwd_async, x.get_device(), xr.data_ptr(), xs, st.shape[0], x.shape[-1],
-                   _TYPES[x.dtype], _ptr(mask), ctx.ms, ctx.temperature, _ptr(tokens), ctx.n, _ptr(logprobs), st.data_ptr(),
+                   _TYPES[x.dtype], _ptr(mr), ms, ctx.temperature, _ptr(tokens), ctx.n, _ptr(logprobs), st.data_ptr(),
                    entropy.data_ptr(), _ptr(dlogp), _ptr(dent), dx.data_ptr()), "token log probabilities backward")
     return dx, None, None, None, None
 
@@ -210,9 +216,9 @@ _logp_backward_once = torch.autograd.function.once_differentiable(_logp_backward
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, mask, temperature, top):
-        logprobs, entropy, st, tl, tt, (xr, mr, ms, n) = _logp_forward(logits, tokens, mask, temperature, top, True)
+        logprobs, entropy, st, tl, tt, (xr, mr, n) = _logp_forward(logits, tokens, mask, temperature, top, True)
         ctx.save_for_backward(xr, tokens, mr, logprobs, st, entropy)
-        ctx.ms, ctx.n, ctx.temperature, ctx.shape = ms, n, temperature, logits.shape
+        ctx.n, ctx.temperature, ctx.shape = n, temperature, logits.shape
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(tl, tt)

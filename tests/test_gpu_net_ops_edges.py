@@ -129,6 +129,27 @@ def test_results_do_not_depend_on_a_common_offset(vocab, dtype):
         assert ref.off(dx, want, tol) <= 1
 
 
+@pytest.mark.parametrize("vocab", [39, 3000])
+def test_gradients_through_saved_tensors_on_the_host(vocab):
+    """torch.autograd.graph.save_on_cpu, which hands dense copies of strided rows and masks back."""
+    from master_doko_reinforcement_learning_amd import layer_norm, token_logprobs
+    g = _gen(vocab)
+    x, delta = (_randn(g, 30, vocab + 10)[:, 4:4 + vocab] for _ in range(2))
+    marks = torch.rand(30, vocab + 5, generator=g, device=DEV) < 0.5
+    t = torch.randint(0, vocab, (30, 2), generator=g, device=DEV)
+    w = _randn(g, vocab, shift=1.0)
+    for mask in (None, marks[:, 2:2 + vocab], marks[3, :vocab], marks[3, :vocab].expand(30, vocab)):
+        outs = []
+        for hooks in (torch.autograd.graph.save_on_cpu, torch.enable_grad):
+            leaves = [u.detach().requires_grad_() for u in (x, delta, w)]
+            with hooks():
+                new, h = layer_norm(leaves[0], leaves[2], delta=leaves[1])
+                got = token_logprobs(h, t, mask=mask)
+            loss = got.logprobs.nan_to_num(neginf=0.0).sum() + got.entropy.sum() + new.sum()
+            outs.append(torch.autograd.grad(loss, leaves))
+        assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
 def test_vocabularies_past_32_bits_are_refused():
     from master_doko_reinforcement_learning_amd import token_logprobs
     one = torch.zeros(1, dtype=BF16, device=DEV)

@@ -122,3 +122,41 @@ def test_layer_norm_entry_refuses_strided_rows_in_place():
         return L.dk_net_layer_norm_async(x, x_stride, delta, delta_stride, 2, 8, 0, None, None, 0, 1e-5, x_out, ctypes.addressof(other) + 1024, None, None)
     assert forward(x_stride=9) == INVALID and forward(x_stride=0) == INVALID and forward(delta=None, x_stride=16) == INVALID
     assert forward(x_out=q, delta_stride=12) == INVALID and forward(x_out=q, delta_stride=0) == INVALID
+
+
+def test_saved_tensors_may_come_back_with_other_strides(monkeypatch):
+    """Saved-tensor hooks (torch.autograd.graph.save_on_cpu) hand back dense copies of strided rows: the backward passes
+    take the strides of what they are given."""
+    from master_doko_reinforcement_learning_amd import net_ops
+    calls = []
+
+    def launch(fn, index, *args):
+        calls.append((fn.__name__,) + args)
+        return 0
+    monkeypatch.setattr(net_ops, "_floating", lambda t, what: net_ops._TYPES[t.dtype])
+    monkeypatch.setattr(net_ops, "_launch", launch)
+    given = {}
+
+    def pack(t):
+        copy = torch.empty(t.shape, dtype=t.dtype)
+        given[copy.data_ptr()] = copy
+        return copy.copy_(t)
+    wide, marks = torch.zeros(6, 50), torch.ones(6, 47, dtype=torch.bool)
+    for mask, strides in ((None, (0,)), (marks[:, 3:43], (40,)), (marks[0, :40], (0,)), (marks[0, :40].expand(6, 40), (0, 40))):
+        x = wide[:, 5:45].requires_grad_()
+        for hooked in (False, True):
+            with torch.autograd.graph.saved_tensors_hooks(pack if hooked else lambda t: t, lambda t: t):
+                got = net_ops.token_logprobs(x, torch.zeros(6, dtype=torch.int64), mask=mask)
+            torch.autograd.grad(got.logprobs.sum(), x)
+            name, logits, stride, rows, vocab, _, m, mask_stride = calls.pop()[:8]
+            assert name == "dk_net_token_logprobs_bwd_async" and (rows, vocab) == (6, 40) and stride == (40 if hooked else 50)
+            if hooked:
+                assert logits in given and (m is None) == (mask is None) and (m is None or m in given) and mask_stride in strides
+            elif mask is not None:
+                assert m == mask.data_ptr() and mask_stride == (0 if mask.dim() == 1 else mask.stride(0))
+    x, w = wide[:, 5:45].requires_grad_(), torch.ones(40)
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        h = net_ops.layer_norm(x, w)
+    torch.autograd.grad(h.sum(), x)
+    name, _, dh_stride, _, _, rows, stride = calls.pop()[:7]
+    assert name == "dk_net_layer_norm_bwd_async" and rows in given and (dh_stride, stride) == (40, 40)
