@@ -475,18 +475,12 @@ struct LogpBwdArgs {
     uint32_t parts;   // of a row
 };
 
-// a row's token i and its gradient (0 and no token for padding, out of range, and what is not allowed or holds -inf).
-// The log probability says which those are, -inf; but in a row with a NaN or +inf every one is NaN, so there the
-// mask and the logit are looked at.
-template <class T>
+// a row's token i and its gradient (0 and no token for padding, out of range, and what is not allowed, whose log
+// probability is -inf; in a row with a NaN or +inf every one is NaN, and so is each allowed entry's gradient without
+// the tokens', while a token that is not allowed could not be told from the others)
 __device__ __forceinline__ float token_gradient(const LogpBwdArgs& a, uint64_t row, uint32_t i, int32_t& token) {
     const int64_t t = a.tokens[row * a.n + i];
-    bool ok = t >= 0 && t < (int64_t)a.vocab;
-    if (ok) {
-        const float lp = a.logprobs[row * a.n + i];
-        ok = lp != NEG_INF;
-        if (lp != lp) ok = (!a.mask || a.mask[row * a.mask_stride + t]) && to_f32(((const T*)a.logits)[row * a.stride + t]) != NEG_INF;
-    }
+    const bool ok = t >= 0 && t < (int64_t)a.vocab && a.logprobs[row * a.n + i] > NEG_INF;
     token = ok ? (int32_t)t : -1;
     return ok ? a.dlogp[row * a.n + i] : 0.0f;
 }
@@ -526,7 +520,7 @@ __global__ __launch_bounds__(256) void token_logprobs_small_bwd_kernel(LogpBwdAr
         float total = 0.0f;
         if (live)
             for (uint32_t i = lane; i < n; i += G) {
-                const float g = token_gradient<T>(a, row, i, tok[slot][i]);
+                const float g = token_gradient(a, row, i, tok[slot][i]);
                 grad[slot][i] = g;
                 total += g;
             }
@@ -576,7 +570,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(LogpBwdArgs a) 
             if (whole) load_logits<T, true>(x, mask, at, a.vocab, v[i]);
             else if (at < a.vocab) load_logits<T, false>(x, mask, at, a.vocab, v[i]);
         }
-        if (tid < n) grad[tid] = token_gradient<T>(a, row, tid, tok[tid]);
+        if (tid < n) grad[tid] = token_gradient(a, row, tid, tok[tid]);
         team_sync<W>();
         float total = 0.0f;
         for (uint32_t k = 0; k < n; ++k) total += grad[k];
