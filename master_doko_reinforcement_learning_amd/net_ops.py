@@ -358,7 +358,8 @@ class AdamW(torch.optim.Optimizer):
                 st["master"].copy_(p)
         # (scratch of a step: the tensors' factors; and the parameters' versions that the masters go with)
         self.buffers.append(b)
-        self._tables.append({"rows": table, "sizes": [p.numel() for p in params], "dtype": params[0].dtype if params else None, "device": dev,
+        self._tables.append({"rows": table, "sizes": list(map(_NUMEL, params)), "memory": list(map(_PTR, params)),
+                             "dtype": params[0].dtype if params else None, "device": dev,
                              "factors": torch.empty(3 * max(1, len(params)), dtype=torch.float32, device=dev),
                              "versions": [p._version for p in params] if master else None})
 
@@ -375,11 +376,11 @@ class AdamW(torch.optim.Optimizer):
     def _step_group(self, group, b, t):
         dtype, device = t["dtype"], t["device"]
         lr, d_lr = _hyper(group)
-        params, sizes, at = group["params"], t["sizes"], None
+        params, sizes, known, at = group["params"], t["sizes"], t["memory"], None
         grads = list(map(_GRAD, params))
         if not all(map(operator.is_not, grads, itertools.repeat(None))):
             at = [i for i, g in enumerate(grads) if g is not None]
-            params, grads, sizes = [params[i] for i in at], [grads[i] for i in at], [sizes[i] for i in at]
+            params, grads, sizes, known = ([u[i] for i in at] for u in (params, grads, sizes, known))
         if not params:
             return
         if d_lr is not None and d_lr.device != device:
@@ -400,11 +401,13 @@ class AdamW(torch.optim.Optimizer):
             self._take_over(t, [(i, p) for i, p in zip(at or range(len(params)), params) if versions[i] != p._version])
         n = len(params)
         rows = t["rows"] if at is None else t["rows"][at]
-        memory = np.fromiter(map(_PTR, params), np.uint64, n)
-        if not np.array_equal(memory, rows["p"]):   # (new memory, through p.data: looked at as the first was)
+        memory = list(map(_PTR, params))
+        if memory != known:   # (new memory, through p.data: looked at as the first was)
             if _overlap(group["params"]):
                 raise RuntimeError("AdamW: a group's parameters overlap since the optimiser was made")
             t["rows"]["p"][slice(None) if at is None else at] = rows["p"] = memory
+            for i, m in zip(at or range(n), memory):
+                t["memory"][i] = m
         rows["g"] = np.fromiter(map(_PTR, grads), np.uint64, n)
         b1, b2 = group["betas"]
         _check(_launch(_native.lib().dk_net_adamw_async, device.index, rows.ctypes.data, n, _TYPES[dtype], self.state_bits,
