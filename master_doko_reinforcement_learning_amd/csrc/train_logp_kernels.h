@@ -10,7 +10,8 @@
 // rounding of a log probability could make ties.
 //
 // Bound by reading the logits (once forward, once backward): an element costs ~11 VALU slots, a quarter
-// of them the exponential, 7 TB/s of bf16 on 256 CUs.
+// of them the exponential, 7 TB/s of bf16 on 256 CUs.  A mask is a byte more for each: 4096 x 65536 bf16 152 us
+// forward and 283 backward against 106 and 245 without, 8000 x 8000 f32 68 and 116 against 50 and 105.
 #pragma once
 #include "train_common.h"
 
@@ -183,7 +184,10 @@ __device__ __forceinline__ void team_sync() {
 // S groups, mine[s] is the largest key of a group; scan(least, push) goes through the groups whose mine is at
 // least `least` and pushes the entries whose key is; best(below) is the thread's largest entry under `below`.
 //   Of a wave's groups at least k have mine >= T for the k-th largest T of them, so no entry below any
-// wave's T is among the k largest: the others are few, except where many are equal.
+// wave's T is among the k largest: the others are few, except where many are equal.  More than ROOM of them (constant
+// rows, a head that is still zero) are taken one after the other, by a pass over the team's entries each: 4096 x 32000
+// f32 of equal logits take 1.87 ms with 20 alternatives and 0.78 ms with 5, of random ones 0.11 and 0.10 ms; 20000 x
+// 1000 bf16 with 20 252 us against 25.
 template <int W, int S>
 struct TopLds {
     static constexpr uint32_t ROOM = W > WAVE ? 1024 : 256;
@@ -354,7 +358,8 @@ __global__ __launch_bounds__(team_threads(W)) void token_logprobs_kernel(LogpArg
             lds.keys[groups++][tid] = order_key(seen);
             seen = NEG_INF;
         }
-        // the rest, less than B vectors a thread: all loads first, then the sums of those that there are
+        // the rest, less than B vectors a thread, those that there are (each load in a branch of its own: those of whole
+        // vectors are in flight together, one with a mask or behind the row's end is waited for)
 #pragma unroll
         for (int i = 0; i < B; ++i)
             if (first + (i * W + tid) * V < hi) load_logits<T, false>(x, mask, first + (i * W + tid) * V, hi, v + i * V);

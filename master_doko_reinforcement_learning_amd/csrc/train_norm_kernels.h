@@ -5,11 +5,13 @@
 //
 // Memory-bound (~10 operations an element forward, ~15 backward), so each pass reads its inputs once: a
 // row lives in the registers of LANES threads, NV 16-byte vectors each, and both reductions (the
-// variance is of differences from the mean, not of squares) run on the registers.
+// variance is of differences from the mean, not of squares) run on the registers.  (Above 12288 columns the
+// backward pass has 12 to 38 registers too few a thread, which go to scratch memory.)
 //   With the residual add, forward / backward (a copy reaches 4.6 TB/s): 31744 x 256 f32 28 us, 4.7 TB/s /
 // 24 us, 5.4 TB/s, and 4 us for the join; 16384 x 4096 bf16 99 us, 5.4 TB/s / 117 us, 4.6 TB/s, and 8 us.
 // Rows of odd width in 16 bits begin between dwords, which costs the cache 20 to 40 %: 50030 x 1111 f16 61 us
-// forward against 51 at 1104 columns, 117 against 85 backward.
+// forward against 51 at 1104 columns, 117 against 85 backward.  Wide rows, with the residual add: 4096 x 12288 f32 169 /
+// 167 us, 4.8 TB/s, bf16 89 / 100, 4.5 and 4.0; 4096 x 16384 f32 220 / 239, 4.9 and 4.5, bf16 123 / 142, 4.4 and 3.8.
 #pragma once
 #include "train_common.h"
 
