@@ -664,7 +664,7 @@ int dk_net_layer_norm_bwd_async(const void* dh, uint64_t dh_stride, const void* 
  * top_tokens are still tokens of the row, NaN never among them).
  * mask_stride 0 applies one mask to every row.  The workspace has dk_net_token_logprobs_workspace bytes
  * (which may be 0: then it may be NULL).
- * dk_net_token_logprobs_bwd_async: dlogits (dense [rows][vocab], of `type`, not the logits' own buffer)
+ * dk_net_token_logprobs_bwd_async: dlogits (dense [rows][vocab], of `type`; the logits' own buffer is refused)
  * from dlogprobs [rows][n] and dentropy [rows] (either may be NULL), with logprobs, stats and entropy of the
  * forward call.  A token given twice takes both gradients; padding, out-of-range and
  * disallowed tokens take none, nor do disallowed entries. */

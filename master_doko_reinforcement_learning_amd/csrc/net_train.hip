@@ -248,7 +248,7 @@ int dk_net_token_logprobs_bwd_async(const void* logits, uint64_t stride, uint64_
         !temperature_ok(temperature))
         return DK_E_INVALID;
     if (rows == 0) return DK_OK;
-    if (!logits || (n && (!tokens || !logprobs)) || !stats || !entropy || !dlogits) return DK_E_INVALID;
+    if (!logits || (n && (!tokens || !logprobs)) || !stats || !entropy || !dlogits || dlogits == logits) return DK_E_INVALID;
     const bool wave = vocab <= LOGP_WAVE;
     const uint32_t unit = (wave ? 64u : 256u) * 4u * (type == DK_F32 ? 4u : 8u), parts = (vocab + unit - 1) / unit;
     const LogpBwdArgs a{logits, stride, rows, vocab, n, mask, mask_stride, 1.0f / temperature, tokens, logprobs, stats, entropy,

@@ -160,3 +160,11 @@ def test_saved_tensors_may_come_back_with_other_strides(monkeypatch):
     torch.autograd.grad(h.sum(), x)
     name, _, dh_stride, _, _, rows, stride = calls.pop()[:7]
     assert name == "dk_net_layer_norm_bwd_async" and rows in given and (dh_stride, stride) == (40, 40)
+
+
+def test_token_logprobs_entry_refuses_the_gradient_over_the_logits():
+    """The tokens' logits are read again after the row's gradients are written."""
+    L = _native.lib()
+    buf, other = ctypes.create_string_buffer(4096), ctypes.create_string_buffer(4096)
+    x, p = ctypes.addressof(buf), ctypes.addressof(other)
+    assert L.dk_net_token_logprobs_bwd_async(x, 8, 1, 8, 0, None, 0, 1.0, p, 1, p, p, p, p, None, x, None) == INVALID
